@@ -133,10 +133,6 @@ def prepare(case, seed):
         s['dy'] = (1e-3 * _activations(gen, case['rows'], case['n'], 'f32')).to(TYPES[case['type']])
     else:
         _prepare_adamw(s, case, gen)
-    if own:      # operands quantised before, as a program keeps them
-        from conv1d_text_vae_amd import fp8
-        for k in set(s) & {'w', 'a', 'b'}:
-            s[k + '8'] = fp8.Fp8Rows(s[k][0], s[k][1].contiguous(), case['k'])
     return s
 
 
@@ -330,9 +326,9 @@ def _run_own(s):
         got = fp8.quantize_both(s['x']) if case['both'] else (fp8.quantize_rows(s['x']),)
         return [t for q in got for t in (q.data, q.scale)]
     if op == 'dense':
-        return fp8.dense(s['x'], s['w8'], s['bias'], relu=case['relu'])
+        return fp8.dense(s['x'], fp8.Fp8Rows(*s['w'], case['k']), s['bias'], relu=case['relu'])
     if op == 'product':
-        return fp8.product(s['a8'], s['b8'], out_dtype=TYPES[case['type']])
+        return fp8.product(fp8.Fp8Rows(*s['a'], case['k']), fp8.Fp8Rows(*s['b'], case['k']), out_dtype=TYPES[case['type']])
     if op == 'linear':
         leaves = [s['x'], s['kernel']] + ([s['bias']] if s['bias'] is not None else [])
         y = fp8.linear(s['x'], s['kernel'], s['bias'])
