@@ -751,10 +751,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fp8_gemm32_kernel(Fp8GemmDev 
     // ---- epilogue (fp32 out where WIDE, else bf16): lane -> row m = lane & 31 of a fragment, columns 8 g + 4 (lane >> 5) .. + 3 for g = 0 .. 3
     char* out = (char*)p.out;
     const int q4 = (lane >> 5) * 4;
+    // every wave has its last fragments in registers, the ring is free (before the branch: at the right edge it parts the waves)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (p.vec16 && n0 + bn + 32 * FN <= p.n) {                     // output rows start on 16-byte boundaries
         // through LDS, 32 rows of the wave at a time, so that the stores are whole runs of a row
         constexpr int PITCH = 32 * FN * 4 + 16;
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         uint8_t* mine = lds + w * 32 * PITCH;
         auto store = [&](auto to_f32, auto with_bias, auto with_relu) {
             constexpr int es = decltype(to_f32)::value ? 4 : 2, lpr = 32 * FN * es / 16, rpi = 64 / lpr;      // lanes a row, rows an instruction

@@ -331,3 +331,39 @@ def test_refusals(fp8):
             bad()
     with pytest.raises(L.C1VError):
         fp8.quantize_rows(torch.zeros(3, 4))
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# operands and sums
+# ---------------------------------------------------------------------------------------------------------------
+def cancelling(m, n, k, seed):
+    """Whole numbers a [m, k], b [n, k] that the quantiser leaves as they are (blocks whose largest value is 448, or 3 at most): in
+    every block of 128 two columns hold 448 * 448 and -448 * 448, which cancel, and the others products of at most 9.  Every
+    partial sum, in any order, is a whole number below 64 * 448^2 < 2^24 for k <= 8192 (or within half of that, 2 * 9 * k, of
+    it), so that fp32 sums are exact; a sum in fewer than 18 bits loses what is left."""
+    rng = np.random.RandomState(seed)
+    a, b = rng.randint(-3, 4, (m, k)).astype(np.float32), rng.randint(-3, 4, (n, k)).astype(np.float32)
+    for kb in range(0, k, 128):
+        w = min(128, k - kb)
+        if w > 1:
+            i, j = kb + rng.choice(w, 2, replace=False)
+            a[:, i] = a[:, j] = 448.0
+            b[:, i], b[:, j] = 448.0, -448.0
+    want = (a.astype(np.float64) @ b.astype(np.float64).T) if m * n * k < 1 << 31 else None
+    a, b = torch.from_numpy(a).cuda(), torch.from_numpy(b).cuda()
+    return a, b, a.double() @ b.double().t() if want is None else torch.from_numpy(want).cuda()
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+@pytest.mark.parametrize('n', [1288, 1304, 1336, 1400, 4104, 4232, 4312])
+def test_right_edges_that_part_the_waves_of_a_workgroup(fp8, kind, n):
+    """Rows on 16-byte boundaries whose last tile some waves cover whole, some in part and some not at all (128 x 128 and
+    256 x 256 tiles); nothing is written behind the last row."""
+    m, k = (2048 if n < 4000 else 4300), 140
+    a, b, want = cancelling(m, n, k, n)
+    assert torch.equal(fp8.product(fp8.quantize_rows(a), fp8.quantize_rows(b), out_dtype=torch.float32), want.float())
+    y = torch.zeros(m + 1, n, dtype=KIND[kind], device='cuda')
+    qa, qb = fp8.quantize_rows(torch.ones(m, k, device='cuda')), fp8.quantize_rows(torch.ones(n, k, device='cuda'))
+    fp8._call('c1v_fp8_gemm', fp8._PRODUCT(qa.data.data_ptr(), qa.scale.data_ptr(), qb.data.data_ptr(), qb.scale.data_ptr(), m, n, 256, 0, 0,
+                                           fp8._CODE[KIND[kind]], y.data_ptr(), n, 0, 0), 0)
+    assert (y[:m] == k).all() and not y[m].any()
