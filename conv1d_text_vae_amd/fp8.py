@@ -62,7 +62,8 @@ def _linear_sizes(*shape_types_needs) -> Tuple[int, int, int]:
 
 class Fp8Rows:
     """A matrix [rows, cols] in 8 bits, its blocks of 128 along the columns: `data` float8_e4m3fn [rows, cols rounded up to
-    128] (zeros behind the last column), `scale` uint8 [blocks, rows rounded up to 16]; value = data * 2^(scale - 127)."""
+    128] (zeros behind the last column), `scale` uint8 [blocks, rows rounded up to 16]; value = data * 2^(scale - 127).
+    Tensors at other strides (a transposition, a slice) are laid out once, here."""
 
     __slots__ = ('data', 'scale', 'cols')
 
@@ -73,9 +74,9 @@ class Fp8Rows:
         if kp != -(-cols // BLOCK) * BLOCK or tuple(scale.shape) != (kp // BLOCK, (rows + 15) // 16 * 16):
             raise ValueError('{0} columns need data [rows, {1}] and scale [{2}, {3}], got {4} and {5}'.format(
                 cols, -(-cols // BLOCK) * BLOCK, -(-cols // BLOCK), (rows + 15) // 16 * 16, tuple(data.shape), tuple(scale.shape)))
-        if not (data.is_contiguous() and scale.is_contiguous()) or data.device != scale.device:
-            raise ValueError('data and scale must be contiguous and on one device')
-        self.data, self.scale, self.cols = data, scale, int(cols)
+        if data.device != scale.device:
+            raise ValueError('data and scale are on {0} and {1}'.format(data.device, scale.device))
+        self.data, self.scale, self.cols = data.contiguous(), scale.contiguous(), int(cols)
 
     @property
     def rows(self) -> int:

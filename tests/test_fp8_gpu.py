@@ -367,3 +367,19 @@ def test_right_edges_that_part_the_waves_of_a_workgroup(fp8, kind, n):
     fp8._call('c1v_fp8_gemm', fp8._PRODUCT(qa.data.data_ptr(), qa.scale.data_ptr(), qb.data.data_ptr(), qb.scale.data_ptr(), m, n, 256, 0, 0,
                                            fp8._CODE[KIND[kind]], y.data_ptr(), n, 0, 0), 0)
     assert (y[:m] == k).all() and not y[m].any()
+
+
+def test_operands_at_any_strides(fp8):
+    """Values and scales as a transposition or a slice leaves them: the constructor lays them out once."""
+    x = data(32, 300, 'f32', 1).clamp(-3, 3)
+    w = fp8.quantize_rows(data(48, 300, 'f32', 2).clamp(-3, 3))
+    want = fp8.dense(x, w)
+    scale = w.scale.t().contiguous().t()
+    wide = torch.zeros(48, 400, dtype=torch.uint8, device='cuda')
+    wide[:, :384] = w.data.view(torch.uint8)
+    values = wide.view(torch.float8_e4m3fn)[:, :384]
+    assert not scale.is_contiguous() and not values.is_contiguous()
+    for v in (fp8.Fp8Rows(w.data, scale, 300), fp8.Fp8Rows(values, w.scale, 300), fp8.Fp8Rows(values, scale, 300)):
+        assert torch.equal(fp8.dense(x, v), want) and torch.equal(fp8.dense(x[:3], v), fp8.dense(x[:3], w))
+        assert torch.equal(fp8.product(fp8.quantize_rows(x), v), fp8.product(fp8.quantize_rows(x), w))
+        assert torch.equal(v.dequantize(), w.dequantize())

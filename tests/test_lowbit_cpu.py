@@ -136,6 +136,23 @@ def test_python_refuses_without_a_gpu():
             f()
 
 
+def test_operands_at_any_strides():
+    """Values and scales as a transposition or a slice leaves them (scales made row by row and transposed, when the number of
+    rows needs no padding, are such)."""
+    from conv1d_text_vae_amd import fp8
+    data = torch.arange(32 * 256).remainder(97).float().view(32, 256).to(torch.float8_e4m3fn)
+    scale = (torch.arange(2 * 32) + 100).to(torch.uint8).view(2, 32)
+    want = fp8.Fp8Rows(data, scale, 200)
+    wide = torch.zeros(32, 300, dtype=torch.uint8)
+    wide[:, :256] = data.view(torch.uint8)
+    values, turned = wide.view(torch.float8_e4m3fn)[:, :256], scale.t().contiguous().t()
+    assert not values.is_contiguous() and not turned.is_contiguous()
+    for q in (fp8.Fp8Rows(data, turned, 200), fp8.Fp8Rows(values, scale, 200), fp8.Fp8Rows(values, turned, 200)):
+        assert q.data.is_contiguous() and q.scale.is_contiguous() and torch.equal(q.scale, scale)
+        assert torch.equal(q.dequantize(), want.dequantize())
+    assert want.data is data and want.scale is scale                      # nothing is copied that needs no copy
+
+
 def test_generator_defaults_are_the_reference_ones():
     from conv1d_text_vae_amd import Conv1dTextVAE
     from conv1d_text_vae_amd.seq2seq import Seq2SeqGenerator

@@ -240,6 +240,41 @@ def test_generator_8bit_weights_per_stream_update_and_graph():
         assert all(torch.equal(a, b) for a, b in zip(out, again))
 
 
+def test_generator_8bit_inference_sees_every_change_of_its_weights():
+    """Updates that the tensors' version counters do not tell -- a replayed optimizer step, a write through `.data`, a replaced
+    `.data` -- between decoded characters: each time the answers of a fresh generator with the same weights."""
+    words, cin, cout = sentences(seed=3)
+    gen, fresh = generator(), generator()
+    h0 = torch.zeros(cin.shape[0], gen.U, device='cuda')
+
+    def check():
+        fresh.set_weights(gen.get_weights())
+        with torch.no_grad():
+            got, want = gen.decode_step(cin[:, :2], h0), fresh.decode_step(cin[:, :2], h0)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            assert torch.equal(gen.encode(words), fresh.encode(words))
+            assert np.array_equal(gen.greedy_decode(got[1], 0, 22, 5), fresh.greedy_decode(want[1], 0, 22, 5))
+        assert torch.equal(gen.eval_batch(words, cin, cout), fresh.eval_batch(words, cin, cout))
+        return got[1]
+    grads = [torch.ones_like(v) for v in gen.p.values()]
+    seen = [check()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gen.opt.step(grads)
+    seen.append(check())
+    assert torch.equal(seen[0], seen[1])                        # (capturing is no step)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        seen.append(check())
+    gen.p['seq2seq_decoder_gru/kernel'].data.mul_(-1.5)
+    seen.append(check())
+    gen.p['seq2seq_decoder_gru/recurrent_kernel'].data = gen.p['seq2seq_decoder_gru/recurrent_kernel'].detach() * 0.5
+    seen.append(check())
+    assert all(not torch.equal(a, b) for a, b in zip(seen[1:], seen[2:]))
+
+
 @pytest.mark.parametrize('products', ['f32', 'fp8'])
 @pytest.mark.parametrize('optimizer', ['adamw', 'adamw8'])
 def test_generator_trains_with_adamw(products, optimizer):

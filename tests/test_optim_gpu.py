@@ -361,3 +361,44 @@ def test_refusals(optim):
             bad()
     with pytest.raises(L.C1VError):
         optim.AdamW([torch.zeros(4)])
+
+
+@pytest.mark.parametrize('states', ['f32', '8bit'])
+def test_states_beside_moments_that_are_no_numbers(optim, states):
+    """Without the clip: NaN, infinities and a square that overflows at every place of a group of four bytes and before the padding;
+    every other state of their blocks to the bit, then a step from what is held.  (The sign of a NaN is nobody's business.)"""
+    n = 300
+    bad = {4: float('nan'), 9: float('inf'), 14: float('-inf'), 19: 3e19, 130: 3e19, 133: float('nan'), 160: float('nan'), 163: -3e19, 299: float('inf')}
+    g = torch.linspace(-1, 1, n).double() ** 3
+    g[5], g[10], g[131] = 0.0, 1e-12, 0.0
+    for i, x in bad.items():
+        g[i] = x
+    first, second = g.float().cuda(), torch.linspace(1, -1, n, device='cuda')
+    opt = optim.AdamW([torch.ones(n, device='cuda')], lr=0.1, weight_decay=0.1, states=states, seed=5)
+    for t, grad in ((1, first), (2, second), (3, second)):
+        before, p0 = held(opt)[0], f64(opt.params[0])
+        opt.step([grad])
+        gp = np.zeros(384, dtype=np.float32)
+        gp[:n] = f32(grad)
+        m, v = O.moments(before[0], before[1], gp, np.float32(1.0), *opt.betas)
+        if states == '8bit':
+            r = O.halves(384, opt.seed, t)
+            cm, sm = O.pack_m(m, r)
+            cv, sv = O.pack_v(v, r)
+            got = opt.m.view(torch.uint8).cpu().numpy()
+            np.testing.assert_array_equal(opt.m_scale.cpu().numpy(), sm)
+            np.testing.assert_array_equal(opt.v_scale.cpu().numpy(), sv)
+            np.testing.assert_array_equal(np.where(np.isnan(m), got & 0x7F, got), np.where(np.isnan(m), cm & 0x7F, cm))
+            np.testing.assert_array_equal(opt.v.cpu().numpy(), cv)
+        else:
+            np.testing.assert_array_equal(opt.m.cpu().numpy(), m)
+            np.testing.assert_array_equal(opt.v.cpu().numpy(), v)
+        m, v = m[:n].astype(np.float64), v[:n].astype(np.float64)
+        with np.errstate(all='ignore'):
+            u = 0.1 * (m / (1 - 0.9 ** t)) / (np.sqrt(v / (1 - 0.999 ** t)) + opt.eps)
+            want = p0 * (1 - 0.1 * 0.1) - u
+            tol = 4 * 2.0 ** -24 * np.abs(p0) + 10 * 2.0 ** -23 * np.abs(u) + 2.0 ** -150 / opt.eps
+        got = f64(opt.params[0])
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        fine = np.isfinite(want)
+        assert fine.sum() >= n - len(bad) and (np.abs(got - want)[fine] <= tol[fine]).all()
