@@ -6,14 +6,11 @@
 // directions.  Scales lie block-major ([block][rows rounded up to 16], 127 behind the last row): one K step of a tile reads
 // them as one contiguous run.
 //
-// Two ways to multiply, chosen by the OUTPUT type:
-//  * bf16 out: v_mfma_scale_f32_16x16x128_f8f6f4 covers one block per instruction and applies both scales inside, at twice
-//    the bf16 rate.  The 8-bit matrix instructions add each group of eight products in a window of 13 bits below the group's
-//    largest product (measured: of 1 + 2^-13 the small part stays, of 1 + 2^-14 it is lost; the groups' sums are then added
-//    in fp32).  An output is off by at most 7 * 2^-13 of its sum of magnitudes and 1.5e-5 to 6.6e-5 in the 2-norm, a
-//    hundredth of what the rounding to bf16 (1.7e-3) does to it.
-//  * fp32 out: the values are widened to bf16 with their scale applied (v_cvt_scalef32_pk_bf16_fp8, exact: e4m3 has four
-//    significant bits) and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are fp32 throughout (1e-8 to 2e-7).
+// Sums are fp32.  The 8-bit matrix instructions do not give them: they add each group of eight products in a window of 13 bits
+// below the group's largest one (measured: of 1 + 2^-13 the small part stays, of 1 + 2^-14 it is lost), so that outputs whose
+// large products cancel lose what is left.  The values are therefore widened to bf16 with their scale applied
+// (v_cvt_scalef32_pk_bf16_fp8, exact: e4m3 has four significant bits) and multiplied by v_mfma_f32_*_bf16, whose products are
+// exact and whose sums are fp32 throughout, at half the 8-bit rate; one rounding to the output's type comes at the end.
 #include <type_traits>
 #include "c1v_common.h"
 
@@ -515,8 +512,8 @@ __device__ __forceinline__ void tile_of(const Fp8GemmDev& p, int bid, int& tm, i
 // DMA.  An operand row of a step is 128 bytes = eight 16-byte pieces; piece c of row r lies at position c ^ ((r >> 1) & 7), so
 // that the 16 rows that a fragment read touches fall on different banks.  b is the MFMA's A operand: a lane then holds four
 // consecutive outputs n of one row m.  For shapes with too few tiles to fill the chip with larger ones; what bounds it is the
-// time of a step's trip through memory and LDS (2048 x 1024 x 384: 6.2 us, 1024 x 1024 x 1024: 6.4 us bf16 out, 7.7 us fp32).
-template <bool WIDE, int BM, int BN, int WM, int WN, int NS>
+// time of a step's trip through memory and LDS (2048 x 1024 x 384: 5.7 us, 1024 x 1024 x 1024: 6.9 us).
+template <int BM, int BN, int WM, int WN, int NS>
 __device__ __forceinline__ void gemm_body(const Fp8GemmDev& p, const int tile, const int split, uint8_t* lds) {
     constexpr int NW = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, J = (BM + BN) / 8 / NW, JA = BM / 8 / NW;
     constexpr int SC = (BM + BN) * 128, STAGE = SC + 512;          // scales of a step: 256 bytes for each operand
@@ -572,29 +569,14 @@ __device__ __forceinline__ void gemm_body(const Fp8GemmDev& p, const int tile, c
         else wait_vm_barrier<0>();
         if (kt + NS - 1 < nk) issue(slot == 0 ? NS - 1 : slot - 1, kt + NS - 1);
         const uint8_t* st = lds + slot * STAGE;
-        if constexpr (WIDE) {
-            Wide bf[FN];
+        Wide bf[FN];
 #pragma unroll
-            for (int j = 0; j < FN; ++j) bf[j] = widen(frag(st, BM + bn + j * 16), st[SC + 256 + bn + j * 16 + fr]);
+        for (int j = 0; j < FN; ++j) bf[j] = widen(frag(st, BM + bn + j * 16), st[SC + 256 + bn + j * 16 + fr]);
 #pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                const Wide af = widen(frag(st, am + i * 16), st[SC + am + i * 16 + fr]);
+        for (int i = 0; i < FM; ++i) {
+            const Wide af = widen(frag(st, am + i * 16), st[SC + am + i * 16 + fr]);
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mfma_wide(bf[j], af, acc[i][j]);
-            }
-        } else {
-            i32x8_t bf[FN];
-            int bs[FN];
-#pragma unroll
-            for (int j = 0; j < FN; ++j) { bf[j] = frag(st, BM + bn + j * 16); bs[j] = st[SC + 256 + bn + j * 16 + fr]; }
-#pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                const i32x8_t af = frag(st, am + i * 16);
-                const int as = st[SC + am + i * 16 + fr];
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[j], af, acc[i][j], 0, 0, 0, bs[j], 0, as);
-            }
+            for (int j = 0; j < FN; ++j) acc[i][j] = mfma_wide(bf[j], af, acc[i][j]);
         }
         slot = slot + 1 == NS ? 0 : slot + 1;
     }
@@ -611,34 +593,33 @@ __device__ __forceinline__ void gemm_body(const Fp8GemmDev& p, const int tile, c
             }
         }
 }
-template <bool WIDE, int BM, int BN, int WM, int WN, int NS>
+template <int BM, int BN, int WM, int WN, int NS>
 __global__ __launch_bounds__(64 * WM * WN, 1) void fp8_gemm_kernel(Fp8GemmDev p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    gemm_body<WIDE, BM, BN, WM, WN, NS>(p, blockIdx.x, blockIdx.y, lds);
+    gemm_body<BM, BN, WM, WN, NS>(p, blockIdx.x, blockIdx.y, lds);
 }
 
 // The two products of a small layer's backward pass and the column sums of its bias gradient in one launch: none of the three
 // fills the chip, and they do not depend on each other (2048 x 302 -> 1024: 8 + 11 + 2 us one after the other).
 struct Fp8PairDev { Fp8GemmDev g[2]; int blocks0, blocks1; const float* part; int64_t tiles, cols; float* sum; };
-template <bool WIDE0, bool WIDE1>
 __global__ __launch_bounds__(256, 1) void fp8_gemm_pair_kernel(Fp8PairDev p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int b = blockIdx.x;
-    if (b < p.blocks0) gemm_body<WIDE0, 64, 64, 2, 2, 4>(p.g[0], b, 0, lds);
-    else if (b < p.blocks0 + p.blocks1) gemm_body<WIDE1, 64, 64, 2, 2, 4>(p.g[1], b - p.blocks0, 0, lds);
+    if (b < p.blocks0) gemm_body<64, 64, 2, 2, 4>(p.g[0], b, 0, lds);
+    else if (b < p.blocks0 + p.blocks1) gemm_body<64, 64, 2, 2, 4>(p.g[1], b - p.blocks0, 0, lds);
     else colsum_body<4>(p.part, p.tiles, p.cols, p.sum, b - p.blocks0 - p.blocks1, (float*)lds);
 }
 
-// Large shapes.  Wave tiles of 32 FM x 32 FN from 32 x 32 matrix instructions (v_mfma_scale_f32_32x32x64_f8f6f4: half the
-// operand registers read per product of the 16 x 16 form), a K step of 128 in two halves of 64: the
-// fragments of one half are read from LDS while the MFMAs of the other run, and the barrier of a step lies between its
-// halves, when the other stage of the two-stage ring has landed and this stage's last fragments are in registers -- the
-// matrix unit has half a step of work queued on either side of it.  Measured: bf16 out 8192^3 508 us (2.17 PFLOP/s), 4096^3 59 us,
-// 16384 x 4096 x 2048 124 us; fp32 out 8192^3 815 us (1.35), 2048 x 4096 x 16384 226 us.  With random operands the limit is
-// the chip's power: the same instructions without any memory traffic reach 3.7 PFLOP/s on them and 4.8 on zeros.
+// Large shapes.  Wave tiles of 32 FM x 32 FN from 32 x 32 matrix instructions (v_mfma_f32_32x32x16_bf16: half the operand
+// registers read per product of the 16 x 16 form), a K step of 128 in two halves of 64: the fragments of one half are read from
+// LDS, as bytes, while the others are widened and multiplied, and the barrier of a step lies between its halves, when the other
+// stage of the two-stage ring has landed and this stage's last fragments are in registers -- the matrix unit has half a step of
+// work queued on either side of it.  Measured, us, bf16 / fp32 out: 8192^3 791 / 815 (1.39 / 1.35 PFLOP/s, a library's bf16
+// product of that size 1.35), 4096^3 104 / 109, 16384 x 4096 x 2048 218 / 235, 2048 x 4096 x 16384 231 / 234.  Bound by the bf16
+// matrix rate; what the 8-bit instructions would save (8192^3 in 450 us) costs the fp32 sums.
 // The outputs of a tile leave through LDS as whole 16-byte pieces of rows; the epilogue is compiled for each combination of bias and
-// relu, and loads the bias once per wave (inline branches per element: 16384 x 4096 x 2048 took 133 us).
-template <bool WIDE, int FM, int FN, int WM, int WN>
+// relu, and loads the bias once per wave (inline branches per element cost 16384 x 4096 x 2048 9 us more).
+template <bool F32, int FM, int FN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 1) void fp8_gemm32_kernel(Fp8GemmDev p) {
     constexpr int BM = 32 * FM * WM, BN = 32 * FN * WN, NW = WM * WN, J = (BM + BN) / 8 / NW, JA = BM / 8 / NW;
     constexpr int SC = (BM + BN) * 128, STAGE = SC + 512;
@@ -705,24 +686,16 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fp8_gemm32_kernel(Fp8GemmDev 
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
     auto multiply = [&](const Half& h, const Scales& s) {
-        if constexpr (WIDE) {
-            Wide bw[FN];
+        Wide bw[FN];
 #pragma unroll
-            for (int j = 0; j < FN; ++j) bw[j] = widen(h.b[j], s.b[j]);
+        for (int j = 0; j < FN; ++j) bw[j] = widen(h.b[j], s.b[j]);
 #pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                const Wide aw = widen(h.a[i], s.a[i]);
+        for (int i = 0; i < FM; ++i) {
+            const Wide aw = widen(h.a[i], s.a[i]);
 #pragma unroll
-                for (int j = 0; j < FN; ++j)
+            for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bw[j].v[q], aw.v[q], acc[i][j], 0, 0, 0);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(h.b[j], h.a[i], acc[i][j], 0, 0, 0, s.b[j], 0, s.a[i]);
+                for (int q = 0; q < 4; ++q) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bw[j].v[q], aw.v[q], acc[i][j], 0, 0, 0);
         }
     };
     issue(0, 0);
@@ -748,7 +721,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fp8_gemm32_kernel(Fp8GemmDev 
     load(y, (nk - 1) & 1, 1);
     multiply(x, sx);
     multiply(y, sx);
-    // ---- epilogue (fp32 out where WIDE, else bf16): lane -> row m = lane & 31 of a fragment, columns 8 g + 4 (lane >> 5) .. + 3 for g = 0 .. 3
+    // ---- epilogue (F32: fp32 out, else bf16): lane -> row m = lane & 31 of a fragment, columns 8 g + 4 (lane >> 5) .. + 3 for g = 0 .. 3
     char* out = (char*)p.out;
     const int q4 = (lane >> 5) * 4;
     // every wave has its last fragments in registers, the ring is free (before the branch: at the right edge it parts the waves)
@@ -791,12 +764,12 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fp8_gemm32_kernel(Fp8GemmDev 
                 wave_lds_sync();
             }
         };
-        const std::bool_constant<WIDE> wide{};
+        const std::bool_constant<F32> f32{};
         const std::true_type yes{};
         const std::false_type no{};
-        if (p.bias) { if (p.relu) store(wide, yes, yes); else store(wide, yes, no); }
-        else if (p.relu) store(wide, no, yes);
-        else store(wide, no, no);
+        if (p.bias) { if (p.relu) store(f32, yes, yes); else store(f32, yes, no); }
+        else if (p.relu) store(f32, no, yes);
+        else store(f32, no, no);
         return;
     }
 #pragma unroll
@@ -844,36 +817,38 @@ static int launch_tiles(const void* f, Fp8GemmDev& p, int bm, int bn, int thread
     }
     return 0;
 }
-template <bool WIDE, int BM, int BN, int WM, int WN, int NS>
+template <int BM, int BN, int WM, int WN, int NS>
 static int launch_gemm(Fp8GemmDev& p, hipStream_t st) {
     constexpr int bytes = NS * ((BM + BN) * 128 + 512);
     static_assert(bytes <= 160 * 1024, "LDS");
     static thread_local int set = -1;
-    return launch_tiles((const void*)fp8_gemm_kernel<WIDE, BM, BN, WM, WN, NS>, p, BM, BN, 64 * WM * WN, bytes, &set, st);
+    return launch_tiles((const void*)fp8_gemm_kernel<BM, BN, WM, WN, NS>, p, BM, BN, 64 * WM * WN, bytes, &set, st);
 }
-template <bool WIDE, int FM, int FN, int WM, int WN>
+template <bool F32, int FM, int FN, int WM, int WN>
 static int launch_gemm32(Fp8GemmDev& p, hipStream_t st) {
     constexpr int BM = 32 * FM * WM, BN = 32 * FN * WN, ring = 2 * ((BM + BN) * 128 + 512), rows = WM * WN * 32 * (32 * FN * 4 + 16), bytes = ring > rows ? ring : rows;
     static_assert(bytes <= 160 * 1024, "LDS");
     static thread_local int set = -1;
-    return launch_tiles((const void*)fp8_gemm32_kernel<WIDE, FM, FN, WM, WN>, p, BM, BN, 64 * WM * WN, bytes, &set, st);
+    return launch_tiles((const void*)fp8_gemm32_kernel<F32, FM, FN, WM, WN>, p, BM, BN, 64 * WM * WN, bytes, &set, st);
 }
 
 struct Fp8Plan { int tile; int splits; };
-// Which kernel, by the work there is for 256 CUs (us, measured with operands in cache; tiles 64: 16 x 16 instructions, four
-// stages; 128: two workgroups per CU; 256: eight waves, one workgroup per CU, 2.1 - 2.4 PFLOP/s where it fills the chip):
-//   2048 x 1024 x 384    64: 7.4   128: 7.5   256: 12      16384 x 4096 x 2048   128: 149   256: 124
-//   1024 x 1024 x 1024   64: 8.3   128: 9.5   256: 19      2048 x 4096 x 16384   128: 115   256: 170 (half the chip)
-//   2048 x 2048 x 2048   64: 21    128: 13    256: 30      8192 x 8192 x 8192    128: 585   256: 508
-// The 128 / 256 choice compares rounds of workgroups times steps (0.93 us a step with 512 slots, 1.6 us with 256) plus 6 / 8 us
+// Which kernel, by the work there is for 256 CUs (us, bf16 out, operands in cache; tiles 64: 16 x 16 instructions, four stages;
+// 128: two workgroups per CU; 256: eight waves, one workgroup per CU):
+//   2048 x 1024 x 384    64: 5.7   128: 6.6   256: 12      4096 x 2048 x 640     128: 14    256: 19
+//   1024 x 1024 x 1024   64: 6.9   128: 11    256: 23      4096 x 4096 x 4096    128: 120   256: 104
+//   2048 x 1024 x 2048   64: 15    128: 18    256: 42      16384 x 4096 x 2048   128: 241   256: 218
+//   2048 x 1300 x 640    64: 10.3  128: 10.1  256: 20      2048 x 4096 x 16384   128: 234   256: 306 (half the chip)
+//   2048 x 2048 x 2048   64: 29    128: 21    256: 44      8192 x 8192 x 8192    128: 890   256: 808
+// The 128 / 256 choice compares rounds of workgroups times steps (1.7 us a step with 512 slots, 3.0 us with 256) plus 6 / 8 us
 // a round.  A long K of few tiles is cut into up to four runs whose fp32 sums a second launch adds in order (512 x 512 x 8192:
-// 25 us whole, 13 us in four; 256 x 512 x 1920: 8.8 us whole, 10.9 us in four).
+// 32 us whole, 14.5 us in four; 512 x 1024 x 8192: 32 us whole, 21.5 in two).
 static Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t kp) {
     const int64_t nk = kp / FB;
     const int64_t t64 = c1v_cdiv(m, 64) * c1v_cdiv(n, 64), t128 = c1v_cdiv(m, 128) * c1v_cdiv(n, 128), t256 = c1v_cdiv(m, 256) * c1v_cdiv(n, 256);
     Fp8Plan p{0, 1};
     if (t128 >= 160) {
-        const double c128 = (double)c1v_cdiv(t128, 512) * (0.93 * nk + 6), c256 = (double)c1v_cdiv(t256, 256) * (1.6 * nk + 8);
+        const double c128 = (double)c1v_cdiv(t128, 512) * (1.7 * nk + 6), c256 = (double)c1v_cdiv(t256, 256) * (3.0 * nk + 8);
         p.tile = c256 < c128 ? 2 : 1;
         return p;
     }
@@ -911,14 +886,10 @@ extern "C" int c1v_fp8_gemm(const c1v_fp8_gemm_args* a, void* stream) {
     Fp8Plan pl;
     if (gemm_setup(a, p, pl)) return -1;
     hipStream_t st = (hipStream_t)stream;
-    if (a->out_dtype == C1V_BF16) {
-        if (pl.tile == 2) return launch_gemm32<false, 4, 2, 2, 4>(p, st);
-        if (pl.tile == 1) return launch_gemm32<false, 2, 2, 2, 2>(p, st);
-        return launch_gemm<false, 64, 64, 2, 2, 4>(p, st);
-    }
-    if (pl.tile == 2) return launch_gemm32<true, 4, 2, 2, 4>(p, st);
-    if (pl.tile == 1) return launch_gemm32<true, 2, 2, 2, 2>(p, st);
-    return launch_gemm<true, 64, 64, 2, 2, 4>(p, st);
+    const bool f32 = a->out_dtype == C1V_F32;
+    if (pl.tile == 2) return f32 ? launch_gemm32<true, 4, 2, 2, 4>(p, st) : launch_gemm32<false, 4, 2, 2, 4>(p, st);
+    if (pl.tile == 1) return f32 ? launch_gemm32<true, 2, 2, 2, 2>(p, st) : launch_gemm32<false, 2, 2, 2, 2>(p, st);
+    return launch_gemm<64, 64, 2, 2, 4>(p, st);
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -936,9 +907,9 @@ struct Fp8RowsDev {
 // lane holds does not matter as long as both sides agree) and feed the weights from memory straight into the MFMA; the waves'
 // sums meet in LDS in the waves' order.  Lanes of rows that x does not have repeat its last row: their products belong to
 // columns of the result that nobody stores.  F fragments per block share the work of quantising x, which would otherwise cost
-// more than the weights' bytes.  13 x 8192 x 4096 bf16 with the weights from memory: 11.9 us for 34 MB, of which 3.5 are what a
-// launch of one block per wave takes (1 x 4096 x 1024); requesting weights two or three blocks further ahead gained nothing.
-template <typename T, int F, int NW, bool WIDE>
+// more than the weights' bytes.  13 x 8192 x 4096 bf16 with the weights from memory: 11.2 us for 34 MB, of which 3.5 are what a
+// launch of one block per wave takes (1 x 1024 x 1024); requesting weights two or three blocks further ahead gained nothing.
+template <typename T, int F, int NW>
 __global__ __launch_bounds__(64 * NW) void fp8_rows_kernel(Fp8RowsDev d) {
     __shared__ f32x4_t red[NW][F][64];
     const Fp8GemmDev& p = d.p;
@@ -992,15 +963,9 @@ __global__ __launch_bounds__(64 * NW) void fp8_rows_kernel(Fp8RowsDev d) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) { af[i] = (int)v.quad(i, s); af[4 + i] = (int)v2.quad(i, s); }
         if (next < p.nk) rows(next);
-        if constexpr (WIDE) {
-            const Wide aw = widen(af, as);
+        const Wide aw = widen(af, as);
 #pragma unroll
-            for (int f = 0; f < F; ++f) acc[f] = mfma_wide(widen(__builtin_shufflevector(lo[f], hi[f], 0, 1, 2, 3, 4, 5, 6, 7), bs[f]), aw, acc[f]);
-        } else {
-#pragma unroll
-            for (int f = 0; f < F; ++f)
-                acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(lo[f], hi[f], 0, 1, 2, 3, 4, 5, 6, 7), af, acc[f], 0, 0, 0, bs[f], 0, as);
-        }
+        for (int f = 0; f < F; ++f) acc[f] = mfma_wide(widen(__builtin_shufflevector(lo[f], hi[f], 0, 1, 2, 3, 4, 5, 6, 7), bs[f]), aw, acc[f]);
 #pragma unroll
         for (int f = 0; f < F; ++f) { lo[f] = lo2[f]; hi[f] = hi2[f]; bs[f] = bs2[f]; }
     }
@@ -1017,9 +982,9 @@ __global__ __launch_bounds__(64 * NW) void fp8_rows_kernel(Fp8RowsDev d) {
 // Whether x is quantised inside the product's launch.  Up to 16 rows always.  Beyond, a workgroup's K is walked eight blocks at
 // a time and x is quantised again for every 16 to 64 columns, against two launches and 64 x 64 tiles that walk K one block at
 // a time.  Measured (us, f32 / bf16 x, back to back):
-//   256 x 512 x 1920   8.1 / 6.6 here, 12.1 / 9.9 in two launches     512 x 512 x 512    4.5 / 4.0,  6.8 / 6.2
-//   256 x 1024 x 1024  6.4 / 5.4,      8.6 / 7.5                      4096 x 64 x 302    4.5 / 4.6,  6.9 / 6.7
-//   1024 x 1024 x 302  15.3 / 15.2,    7.0 / 6.6 (1024 workgroups)    128 x 512 x 4096   17.2 / 14.3, 11.5 / 10.4 (32 blocks of K)
+//   256 x 512 x 1920   7.9 / 6.4 here, 12.0 / 12.0 in two launches    512 x 512 x 512    4.7 / 4.1,  6.7 / 6.8
+//   256 x 1024 x 1024  6.4 / 5.4,      8.5 / 8.5                      4096 x 64 x 302    4.8 / 4.7,  6.8 / 7.0
+//   1024 x 1024 x 302  15.6 / 14.7,    6.9 / 7.0 (1024 workgroups)    256 x 512 x 4096   13.9 / 10.0, 12.6 / 12.4 (32 blocks of K)
 static bool fp8_dense_direct(int64_t m, int64_t n, int64_t kp) {
     return m <= C1V_FP8_ROWS || (c1v_cdiv(m, 16) * c1v_cdiv(n, 64) <= 256 && kp <= 16 * FB);
 }
@@ -1028,8 +993,7 @@ extern "C" int c1v_fp8_dense_direct(int64_t m, int64_t n, int64_t kp) { return f
 template <typename T, int F>
 static void launch_rows1(const Fp8RowsDev& d, hipStream_t st) {
     const dim3 grid((unsigned)c1v_cdiv(d.p.n, 16 * F), (unsigned)c1v_cdiv(d.rows, 16));
-    if (d.p.out_dtype == C1V_F32) hipLaunchKernelGGL((fp8_rows_kernel<T, F, 8, true>), grid, dim3(512), 0, st, d);
-    else hipLaunchKernelGGL((fp8_rows_kernel<T, F, 8, false>), grid, dim3(512), 0, st, d);
+    hipLaunchKernelGGL((fp8_rows_kernel<T, F, 8>), grid, dim3(512), 0, st, d);
 }
 // One fragment column per workgroup gives the most workgroups, two or four share the work of quantising x and its reads.
 // Measured for up to 16 rows (us, bf16 x, weights from memory):
@@ -1136,18 +1100,17 @@ c1v_fp8_gemm_args linear_gemm(const void* a, const void* sa, const void* b, cons
     g.work = w.work; g.work_bytes = w.work_bytes;
     return g;
 }
-template <bool WIDE0, bool WIDE1>
 int launch_pair(const Fp8PairDev& p, unsigned blocks, hipStream_t st) {
     constexpr int bytes = 4 * ((64 + 64) * 128 + 512);
     static thread_local int set = -1;
     int dev = 0;
     (void)hipGetDevice(&dev);
     if (set != dev) {
-        const hipError_t e = hipFuncSetAttribute((const void*)fp8_gemm_pair_kernel<WIDE0, WIDE1>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        const hipError_t e = hipFuncSetAttribute((const void*)fp8_gemm_pair_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
         C1V_REQUIRE(e == hipSuccess, "fp8_linear_bwd: %s", hipGetErrorString(e));
         set = dev;
     }
-    hipLaunchKernelGGL((fp8_gemm_pair_kernel<WIDE0, WIDE1>), dim3(blocks), dim3(256), bytes, st, p);
+    hipLaunchKernelGGL(fp8_gemm_pair_kernel, dim3(blocks), dim3(256), bytes, st, p);
     C1V_LAUNCH_CHECK();
     return 0;
 }
@@ -1195,8 +1158,7 @@ extern "C" int c1v_fp8_linear_bwd(const c1v_fp8_linear_args* a, void* stream) {
             p.blocks0 = p.g[0].tiles_m * p.g[0].tiles_n; p.blocks1 = p.g[1].tiles_m * p.g[1].tiles_n;
             p.part = b.part; p.tiles = c1v_cdiv(a->rows, FB); p.cols = a->n; p.sum = a->db;
             const unsigned blocks = (unsigned)(p.blocks0 + p.blocks1 + (a->need_db ? c1v_cdiv(a->n, 64) : 0));
-            if (a->x_dtype == C1V_F32) return a->k_dtype == C1V_F32 ? launch_pair<true, true>(p, blocks, st) : launch_pair<true, false>(p, blocks, st);
-            return a->k_dtype == C1V_F32 ? launch_pair<false, true>(p, blocks, st) : launch_pair<false, false>(p, blocks, st);
+            return launch_pair(p, blocks, st);
         }
     }
     int rc = c1v_fp8_quantize(&q, stream);

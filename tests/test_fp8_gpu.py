@@ -2,8 +2,8 @@
 
 Tolerances.  The quantiser is exact: values and scales are compared to the bit.  A product of quantised operands adds K exact
 products (4 + 4 significant bits) in fp32 in some order: off by at most K * 2^-24 * sum_k |a_k b_k|, plus half a step of the output
-type (2^-24 / 2^-8 of the value).  With bf16 outputs the 8-bit matrix instruction adds each group of eight products in a window
-of 13 bits below the largest of them, so seven of the eight lose up to 2^-13 of it: 7 * 2^-13 * sum_k |a_k b_k| more."""
+type (2^-24 / 2^-8 of the value).  `check_product` and the tests before "operands and sums" allow bf16 outputs 7 * 2^-13 *
+sum_k |a_k b_k| more, what the 8-bit matrix instructions would lose; the tests behind it do not: sums are fp32 for every type."""
 import numpy as np
 import pytest
 import torch
@@ -367,6 +367,67 @@ def test_right_edges_that_part_the_waves_of_a_workgroup(fp8, kind, n):
     fp8._call('c1v_fp8_gemm', fp8._PRODUCT(qa.data.data_ptr(), qa.scale.data_ptr(), qb.data.data_ptr(), qb.scale.data_ptr(), m, n, 256, 0, 0,
                                            fp8._CODE[KIND[kind]], y.data_ptr(), n, 0, 0), 0)
     assert (y[:m] == k).all() and not y[m].any()
+
+
+# up to 16 rows (one and two column fragments a workgroup), short batches (one, two, four), 64 x 64 tiles, a K in runs, 128 x 128
+# and 256 x 256 tiles on and off 16-byte boundaries
+SUMS = [(1, 1024, 1024), (13, 8192, 1024), (64, 512, 1920), (256, 512, 1920), (512, 512, 512), (1999, 1021, 302), (1024, 1024, 1024),
+        (512, 512, 8192), (66, 130, 4352), (2048, 2048, 640), (2050, 1301, 300), (4352, 4096, 384), (4100, 4401, 330)]
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+@pytest.mark.parametrize('m,n,k', SUMS)
+def test_sums_are_fp32_whatever_the_output_type(fp8, kind, m, n, k):
+    a, b, want = cancelling(m, n, k, m + n)
+    want = want.float().to(KIND[kind])
+    qa, qb = fp8.quantize_rows(a), fp8.quantize_rows(b)
+    assert torch.equal(qa.dequantize(), a) and torch.equal(qb.dequantize(), b)
+    assert torch.equal(fp8.product(qa, qb, out_dtype=KIND[kind]), want)
+    for x in (a, a.bfloat16()):
+        assert torch.equal(fp8.dense(x, qb, out_dtype=KIND[kind]), want)
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+@pytest.mark.parametrize('m,n,k', [(300, 200, 140), (130, 66, 4300), (2050, 1301, 300), (4352, 4096, 384)])
+def test_sums_of_a_layer_and_its_gradients_are_fp32(fp8, kind, m, n, k):
+    """Each of the three products by itself as the one that cancels (in a small layer both gradients share a launch)."""
+    a, b, want = cancelling(m, n, k, m + n + 1)
+    t = KIND[kind]
+    want = want.float().to(t)
+    a, b = a.to(t), b.to(t)
+    with torch.no_grad():
+        assert torch.equal(fp8.linear(a, b.t()), want)                                          # y = x W
+    for other in (False, True):
+        x, w = torch.ones(m, n, dtype=t, device='cuda').requires_grad_(True), b.t().contiguous().t().requires_grad_(other)
+        dx = torch.autograd.grad(fp8.linear(x, w), x, a, retain_graph=True)[0]                   # dx = dy W^T
+        assert torch.equal(dx, want)
+        x, w = a.t().contiguous().requires_grad_(other), torch.ones(m, n, dtype=t, device='cuda').requires_grad_(True)
+        dw = torch.autograd.grad(fp8.linear(x, w), w, b.t().contiguous())[0]                     # dW = x^T dy
+        assert torch.equal(dw, want)
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+@pytest.mark.parametrize('rows,k,n', [(4100, 60, 4200), (2304, 1408, 1900), (4500, 4400, 520)])
+def test_linear_of_large_layers(fp8, kind, rows, k, n):
+    """Both gradients with a K in runs (one workspace), and through the larger tiles, against 64 bits: K * 2^-24 of the sum of
+    magnitudes and half a step of the output type."""
+    x, w = data(rows, k, kind, 1).clamp(-3, 3).requires_grad_(True), data(k, n, 'f32', 2).clamp(-3, 3).requires_grad_(True)
+    bias = torch.linspace(-1, 1, n, device='cuda').requires_grad_(True)
+    dy = data(rows, n, kind, 3).clamp(-3, 3)
+    y = fp8.linear(x, w, bias)
+    dx, dw, db = torch.autograd.grad(y, (x, w, bias), dy)
+    x, w, bias = x.detach(), w.detach(), bias.detach().double()
+    deq = lambda q: q.dequantize().double()
+    for got, a, b, add in ((y, fp8.quantize_rows(x), fp8.quantize_cols(w), bias), (dx, fp8.quantize_rows(dy), fp8.quantize_rows(w), None),
+                           (dw, fp8.quantize_cols(x), fp8.quantize_cols(dy), None)):
+        A, B = deq(a), deq(b)
+        want, size = A @ B.t(), A.abs() @ B.abs().t()
+        if add is not None:
+            want, size = want + add, size + add.abs()
+        half = 2.0 ** -24 if got.dtype == torch.float32 else 2.0 ** -8
+        assert ((got.double() - want).abs() <= half * want.abs() + (A.shape[1] + 2) * 2.0 ** -24 * size * (1 + half)).all()
+    D = dy.double()
+    assert ((db.double() - D.sum(0)).abs() <= rows * 2.0 ** -24 * D.abs().sum(0)).all()
 
 
 def test_operands_at_any_strides(fp8):
