@@ -224,7 +224,8 @@ template <int B> __device__ __forceinline__ uint32_t pack_m(uint32_t w, float m,
     return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(z, (int)seed, (int)w, B);
 }
 // v: byte c stands for the float with bits (c + 8 s - 240) << 20 (0: zero, 255: NaN); the block's largest value has c in 240 .. 248.
-// base20 = (8 s - 240) << 20.  r2 = another 16 bits from the same r, shifted up by 4, plus 8.
+// base20 = (8 s - 240) << 20.  r2 = another 16 bits from the same r, shifted up by 4, plus 8.  Finite values only: they give eight
+// bits, what is not finite would reach into its neighbours' bytes.
 __device__ __forceinline__ uint32_t pack_v(float v, uint32_t base20, uint32_t r) {
     const uint32_t u = __float_as_uint(v), r2 = (__umul24(r, 40503u << 4) & 0xffff0u) | 8u;
     const int c = (int)(u + r2 - base20) >> 20, least = (int)(u < 1u ? u : 1u);      // 1 for what is not zero
@@ -302,10 +303,15 @@ __global__ __launch_bounds__(256) void adamw_update_kernel(AdamwDev d) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) { um = umax(um, __float_as_uint(m[k]) & 0x7fffffffu); uv = umax(uv, __float_as_uint(v[k]) & 0x7fffffffu); }
             const bool odd = __any(umax(um, uv) >= 0x7f800000u);             // rare: only finite values make the scales
+            uint32_t lost = 0;                                               // which v are no numbers (packed as 0, then marked)
             if (odd) {
                 um = uv = 0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) { um = umax(um, finite_mag(m[k])); uv = umax(uv, finite_mag(v[k])); }
+                for (int k = 0; k < 8; ++k) {
+                    um = umax(um, finite_mag(m[k]));
+                    if ((__float_as_uint(v[k]) & 0x7fffffffu) >= 0x7f800000u) { lost |= 1u << k; v[k] = 0.f; }
+                    uv = umax(uv, __float_as_uint(v[k]));
+                }
             }
             int sm = (int)(row_max(um) >> 23) - 7, sv = (int)(row_max(uv) >> 23);
             sm = sm < 1 ? 1 : sm;
@@ -331,7 +337,7 @@ __global__ __launch_bounds__(256) void adamw_update_kernel(AdamwDev d) {
                     const uint32_t sh = 8 * (k & 3);
                     if ((__float_as_uint(m[k]) & 0x7fffffffu) >= 0x7f800000u)
                         mo[k >> 2] = (mo[k >> 2] & ~(0xffu << sh)) | ((0x7fu | ((__float_as_uint(m[k]) >> 24) & 0x80u)) << sh);
-                    if ((__float_as_uint(v[k]) & 0x7fffffffu) >= 0x7f800000u) vo[k >> 2] |= 0xffu << sh;
+                    if (lost >> k & 1) vo[k >> 2] |= 0xffu << sh;
                 }
             }
             *(uint2*)((uint8_t*)d.m + e) = make_uint2(mo[0], mo[1]);
