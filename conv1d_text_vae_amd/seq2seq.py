@@ -17,8 +17,9 @@ semantics restated here can be unit-tested without a GPU).  What is restated fro
 
 Beside the reference's arithmetic (the default): optimizer='adamw' / 'adamw8' trains with optim.AdamW, one launch over all
 weights, its states in fp32 or in 8 bits; products='fp8' computes the dense products over whole sequences in 8 bits
-(fp8.linear) when training, and every dense product when encoding and decoding (fp8.dense over weights quantised once per
-weight update, the two gates' recurrent kernels in one product).  Both run hand-written kernels and need a GPU.
+(fp8.linear) when training, and every dense product when encoding and decoding without gradients (fp8.dense over weights
+quantised once per call of encode / decode_step / eval_batch / greedy_decode, the two gates' recurrent kernels in one product).
+Both run hand-written kernels and need a GPU.
 """
 from __future__ import annotations
 
@@ -88,7 +89,6 @@ class Seq2SeqGenerator:
                              weight_decay=[0.0 if k.endswith('/bias') else float(weight_decay) for k in self.p],
                              states='8bit' if optimizer == 'adamw8' else 'f32')
         self._opt_lr = self.lr
-        self._served = (None, {})              # 8-bit weights of the inference products, and the weights they were made from
         self.gen = torch.Generator(device=self.dev)
         self.gen.manual_seed(int(seed) + 17)
 
@@ -106,24 +106,15 @@ class Seq2SeqGenerator:
                 self.p[k].copy_(torch.as_tensor(np.asarray(v, dtype=np.float32)))
 
     # ---- products --------------------------------------------------------------------------------------
-    def _weights8(self, name: str, lo: int, hi: int):
-        """Columns [lo, hi) of a kernel in 8 bits, quantised once per update of the weights (torch's version counters tell) and
-        stream that asks: what another stream is still writing is not read, and memory is not reused under its reader.  While a
-        graph is captured they are quantised into it, so that a replay computes with the weights of its time."""
-        from . import fp8
-        make = lambda: fp8.quantize_cols(self.p[name].detach()[:, lo:hi])
-        if self.dev.type != 'cuda' or torch.cuda.is_current_stream_capturing():
-            return make()
-        state = tuple(v._version for v in self.p.values())
-        if self._served[0] != state:
-            self._served = (state, {})
-        held = self._served[1]
-        key = (torch.cuda.current_stream(self.dev).cuda_stream, name, lo, hi)
-        if key not in held:
-            held[key] = make()
-        return held[key]
+    def _weights8(self, name: str, lo: int, hi: int, held: dict):
+        """Columns [lo, hi) of a kernel in 8 bits, quantised once per call (`held` is the call's own).  They are not kept beyond
+        it: nothing tells of a write to the weights through `.data` or of a replayed step of the optimizer."""
+        if (name, lo, hi) not in held:
+            from . import fp8
+            held[name, lo, hi] = fp8.quantize_cols(self.p[name].detach()[:, lo:hi])
+        return held[name, lo, hi]
 
-    def _dense(self, x: torch.Tensor, name: str, bias: Optional[torch.Tensor], lo: int, hi: int, train: bool) -> torch.Tensor:
+    def _dense(self, x: torch.Tensor, name: str, bias: Optional[torch.Tensor], lo: int, hi: int, train: bool, held: dict) -> torch.Tensor:
         """x @ kernel[:, lo:hi] + bias[lo:hi]"""
         W = self.p[name]
         b = None if bias is None else bias[lo:hi]
@@ -132,7 +123,7 @@ class Seq2SeqGenerator:
             if torch.is_grad_enabled():
                 return fp8.linear(x, W[:, lo:hi], b)
             if not train:
-                return fp8.dense(x, self._weights8(name, lo, hi), None if b is None else b.detach())
+                return fp8.dense(x, self._weights8(name, lo, hi, held), None if b is None else b.detach())
         y = torch.matmul(x, W[:, lo:hi])
         return y if b is None else y + b
 
@@ -142,7 +133,7 @@ class Seq2SeqGenerator:
         a = torch.softmax(torch.matmul(x.transpose(1, 2), self.p['attention_aux3/kernel']), dim=-1)      # [B, F, T]
         return x * a.mean(dim=1).unsqueeze(-1)
 
-    def _gru(self, name: str, x: torch.Tensor, h0: torch.Tensor, masked: bool, train: bool, return_sequences: bool):
+    def _gru(self, name: str, x: torch.Tensor, h0: torch.Tensor, masked: bool, train: bool, return_sequences: bool, held: dict):
         W, U, b = self.p[name + '/kernel'], self.p[name + '/recurrent_kernel'], self.p[name + '/bias']
         B, T, _ = x.shape
         u = self.U
@@ -153,12 +144,12 @@ class Seq2SeqGenerator:
                 return keep / (1.0 - rate)
             dp = [drop((B, 1, x.shape[2]), GRU_DROPOUT) for _ in range(3)]
             rdp = [drop((B, u), GRU_RECURRENT_DROPOUT) for _ in range(3)]
-            xz = self._dense(x * dp[0], name + '/kernel', b, 0, u, train)
-            xr = self._dense(x * dp[1], name + '/kernel', b, u, 2 * u, train)
-            xh = self._dense(x * dp[2], name + '/kernel', b, 2 * u, 3 * u, train)
+            xz = self._dense(x * dp[0], name + '/kernel', b, 0, u, train, held)
+            xr = self._dense(x * dp[1], name + '/kernel', b, u, 2 * u, train, held)
+            xh = self._dense(x * dp[2], name + '/kernel', b, 2 * u, 3 * u, train, held)
         else:
             rdp = None
-            xw = self._dense(x, name + '/kernel', b, 0, 3 * u, train)
+            xw = self._dense(x, name + '/kernel', b, 0, 3 * u, train, held)
             xz, xr, xh = xw[..., :u], xw[..., u:2 * u], xw[..., 2 * u:]
         Uz, Ur, Uh = U[:, :u], U[:, u:2 * u], U[:, 2 * u:]
         h = h0
@@ -166,10 +157,10 @@ class Seq2SeqGenerator:
         served = self.products == 'fp8' and not train and not torch.is_grad_enabled()
         for t in range(T):
             if served:
-                hzr = self._dense(h, name + '/recurrent_kernel', None, 0, 2 * u, False)
+                hzr = self._dense(h, name + '/recurrent_kernel', None, 0, 2 * u, False, held)
                 z = hard_sigmoid(xz[:, t] + hzr[:, :u])
                 r = hard_sigmoid(xr[:, t] + hzr[:, u:])
-                hh = torch.tanh(xh[:, t] + self._dense(r * h, name + '/recurrent_kernel', None, 2 * u, 3 * u, False))
+                hh = torch.tanh(xh[:, t] + self._dense(r * h, name + '/recurrent_kernel', None, 2 * u, 3 * u, False, held))
                 h_new = z * h + (1.0 - z) * hh
                 h = h_new if mask is None else torch.where(mask[:, t].unsqueeze(-1), h_new, h)
                 if return_sequences:
@@ -191,20 +182,23 @@ class Seq2SeqGenerator:
         """generator_encoder_ (:1309): reconstructed word vectors [B, T, F] -> GRU state [B, units]."""
         x = self.attention(word_vectors) if self.use_attention else word_vectors
         h0 = torch.zeros((x.shape[0], self.U), dtype=x.dtype, device=x.device)
-        _, h, _ = self._gru('seq2seq_encoder_gru', x, h0, masked=True, train=train, return_sequences=False)
+        _, h, _ = self._gru('seq2seq_encoder_gru', x, h0, masked=True, train=train, return_sequences=False, held={})
         return h
 
     def decode_step(self, chars_onehot: torch.Tensor, state: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """generator_decoder_ (:1311-1318): ([B, L, C] one-hot, [B, units]) -> (softmax [B, L, C], new state)."""
-        seq, h, _ = self._gru('seq2seq_decoder_gru', chars_onehot, state, masked=False, train=False, return_sequences=True)
-        logits = self._dense(seq, 'seq2seq_decoder_dense/kernel', self.p['seq2seq_decoder_dense/bias'], 0, self.C, False)
+        return self._decode_step(chars_onehot, state, {})
+
+    def _decode_step(self, chars_onehot: torch.Tensor, state: torch.Tensor, held: dict) -> Tuple[torch.Tensor, torch.Tensor]:
+        seq, h, _ = self._gru('seq2seq_decoder_gru', chars_onehot, state, masked=False, train=False, return_sequences=True, held=held)
+        logits = self._dense(seq, 'seq2seq_decoder_dense/kernel', self.p['seq2seq_decoder_dense/bias'], 0, self.C, False, held)
         return torch.softmax(logits, dim=-1), h
 
     def loss(self, word_vectors: torch.Tensor, dec_in: torch.Tensor, dec_target: torch.Tensor, train: bool) -> torch.Tensor:
         """seq2seq_model_for_training (:1327) with Keras' masked categorical cross-entropy."""
-        state = self.encode(word_vectors, train=train)
-        seq, _, mask = self._gru('seq2seq_decoder_gru', dec_in, state, masked=True, train=train, return_sequences=True)
-        p = torch.softmax(self._dense(seq, 'seq2seq_decoder_dense/kernel', self.p['seq2seq_decoder_dense/bias'], 0, self.C, train), dim=-1)
+        state, held = self.encode(word_vectors, train=train), {}
+        seq, _, mask = self._gru('seq2seq_decoder_gru', dec_in, state, masked=True, train=train, return_sequences=True, held=held)
+        p = torch.softmax(self._dense(seq, 'seq2seq_decoder_dense/kernel', self.p['seq2seq_decoder_dense/bias'], 0, self.C, train, held), dim=-1)
         p = p / p.sum(dim=-1, keepdim=True)
         p = torch.clamp(p, 1e-7, 1.0 - 1e-7)
         xent = -(dec_target * torch.log(p)).sum(dim=-1)                                  # [B, L]
@@ -257,9 +251,10 @@ class Seq2SeqGenerator:
         done = torch.zeros((B,), dtype=torch.bool, device=state.device)
         out = torch.full((B, max_chars + 1), int(eos_idx), dtype=torch.int64, device=state.device)
         eye = torch.eye(self.C, dtype=state.dtype, device=state.device)
+        held: dict = {}                                               # one quantisation of the weights for all characters
         check_every = 16
         for step in range(max_chars + 1):
-            probs, state = self.decode_step(eye[cur].unsqueeze(1), state)
+            probs, state = self._decode_step(eye[cur].unsqueeze(1), state, held)
             cur = torch.argmax(probs[:, -1, :], dim=1)                # first maximum wins, as np.argmax (:457)
             out[:, step] = torch.where(done, out[:, step], cur)
             done = done | (cur == eos_idx)
