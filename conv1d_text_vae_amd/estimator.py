@@ -37,6 +37,8 @@ EPSILON = 1e-7                    # keras.backend.epsilon()
 FITTED_ATTRIBUTES = ['input_text_size_', 'output_text_size_', 'input_vector_size_', 'output_vector_size_',
                      'vae_encoder_', 'vae_decoder_', 'generator_encoder_', 'generator_decoder_',
                      'output_text_size_in_characters_', 'target_char_index_', 'reverse_target_char_index_']
+# how the two stages are computed: attributes beside the parameters, pickled with them
+COMPUTE_CHOICES = ('vae_optimizer', 'generator_optimizer', 'generator_products')
 # layers of 'EncoderForVAE' = Model(encoder_input, z_mean) (:1308): what `vae_encoder_` saves, pickles and hands to a warm start.
 # The z_log_var head belongs to neither saved model: after unpickling / in a warm start it is freshly initialised, as in the
 # reference (whose rebuilt graph gives it new random weights, frozen in a warm start, :1245).
@@ -1092,7 +1094,9 @@ class Conv1dTextVAE(BaseEstimator, TransformerMixin, ClassifierMixin):
         state = self.get_params(deep=False)
         state.pop('input_embeddings', None)
         state.pop('output_embeddings', None)
+        state.update({name: getattr(self, name) for name in COMPUTE_CHOICES})
         if all(hasattr(self, it) for it in FITTED_ATTRIBUTES):
+            state['generator_products_'] = self.generator_encoder_.gen.products       # (as fitted, whatever was chosen since)
             for name in ('input_text_size_', 'output_text_size_', 'input_vector_size_', 'output_vector_size_',
                          'output_text_size_in_characters_'):
                 state[name] = getattr(self, name)
@@ -1117,6 +1121,9 @@ class Conv1dTextVAE(BaseEstimator, TransformerMixin, ClassifierMixin):
                                                'output_vector_size_', 'weights_', 'output_text_size_in_characters_',
                                                'target_char_index_', 'reverse_target_char_index_'])
         self.set_params(**state)
+        for name in COMPUTE_CHOICES:                                   # (states of before these choices: the class's own)
+            if name in state:
+                setattr(self, name, state[name])
         if is_fitted:
             if not isinstance(state['weights_'], dict):
                 raise ValueError('Weights are wrong! Expected `{0}`, got `{1}`.'.format(type({'a': 1, 'b': 2}),
@@ -1135,6 +1142,7 @@ class Conv1dTextVAE(BaseEstimator, TransformerMixin, ClassifierMixin):
             vae_weights.update(_npz_load(state['weights_']['vae_decoder']))
             runtime, generator = self._create_model(self.input_vector_size_, self.output_vector_size_, seed=0,
                                                     vae_weights=vae_weights)
+            generator.products = state.get('generator_products_', generator.products)
             generator.set_weights(_npz_load(state['weights_']['seq2seq_encoder']))
             generator.set_weights(_npz_load(state['weights_']['seq2seq_decoder']))
             self._vae_runtime = runtime

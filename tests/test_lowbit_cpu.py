@@ -161,6 +161,40 @@ def test_generator_defaults_are_the_reference_ones():
     assert (Conv1dTextVAE.vae_optimizer, Conv1dTextVAE.generator_optimizer, Conv1dTextVAE.generator_products) == ('nadam', 'rmsprop', 'f32')
 
 
+def test_estimator_keeps_its_choices_when_pickled():
+    """Unfitted and fitted; a fitted one serves as it was fitted, whatever was chosen since; states of before load as they did."""
+    import copy
+    import pickle
+    from conv1d_text_vae_amd import Conv1dTextVAE
+    from conv1d_text_vae_amd import estimator as E
+    from conv1d_text_vae_amd.embeddings import synthetic_fasttext
+    emb = synthetic_fasttext(['aa', 'bb'], vector_size=6, bucket=20, seed=1)
+    choices = lambda v: (v.vae_optimizer, v.generator_optimizer, v.generator_products)
+    vae = Conv1dTextVAE(emb, emb, n_filters=4, latent_dim=3, n_recurrent_units=5)
+    assert 'vae_optimizer' not in pickle.loads(pickle.dumps(vae)).get_params() and choices(pickle.loads(pickle.dumps(vae))) == choices(Conv1dTextVAE)
+    vae.vae_optimizer, vae.generator_optimizer, vae.generator_products = 'adamw8', 'adamw', 'fp8'
+    for other in (pickle.loads(pickle.dumps(vae)), copy.deepcopy(vae)):
+        assert choices(other) == ('adamw8', 'adamw', 'fp8')
+    vae.input_text_size_ = vae.output_text_size_ = 4
+    vae.input_vector_size_ = vae.output_vector_size_ = 8
+    vae.output_text_size_in_characters_, vae.target_char_index_, vae.reverse_target_char_index_ = 9, {'a': 0, 'b': 1}, {0: 'a', 1: 'b'}
+    rt, gen = vae._create_model(8, 8, seed=1)
+    vae._vae_runtime, vae._generator = rt, gen
+    vae.vae_encoder_, vae.vae_decoder_ = E.VAEEncoderModel(rt), E.VAEDecoderModel(rt)
+    vae.generator_encoder_, vae.generator_decoder_ = gen.encoder_model(), gen.decoder_model()
+    got = pickle.loads(pickle.dumps(vae))
+    assert choices(got) == ('adamw8', 'adamw', 'fp8')
+    assert (got._generator.products, got._generator.optimizer, got._vae_runtime.optimizer) == ('fp8', 'adamw', 'adamw8')
+    assert all(np.array_equal(v, got._generator.get_weights()[k]) for k, v in gen.get_weights().items())
+    vae.generator_products = 'f32'
+    got = pickle.loads(pickle.dumps(vae))
+    assert got.generator_products == 'f32' and got._generator.products == 'fp8'
+    old = {k: v for k, v in vae.__getstate__().items() if not k.endswith('_optimizer') and not k.startswith('generator_products')}
+    got = Conv1dTextVAE.__new__(Conv1dTextVAE)
+    got.__setstate__(old)
+    assert choices(got) == choices(Conv1dTextVAE) and got._generator.products == 'f32'
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # the oracle
 # ---------------------------------------------------------------------------------------------------------------
