@@ -164,9 +164,17 @@ def _check_bias(bias, n: int, device):
         raise ValueError('bias must be a contiguous float32 vector of {0} values on {1}'.format(n, device))
 
 
+def _no_gradient(what: str):
+    """A product that has no gradient does not drop out of a graph unnoticed."""
+    if torch.is_grad_enabled():
+        raise ValueError('{0} has no gradient, and one of its inputs requires one: use linear, detach() or torch.no_grad()'.format(what))
+
+
 def product(a: Fp8Rows, b: Fp8Rows, bias: Optional[torch.Tensor] = None, relu: bool = False,
             out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """[a.rows, b.rows] = relu(a @ b.T + bias)"""
+    """[a.rows, b.rows] = relu(a @ b.T + bias).  No gradient: a bias that requires one is refused while gradients are enabled."""
+    if bias is not None and bias.requires_grad:
+        _no_gradient('product')
     dev = a.data.device
     if a.cols != b.cols:
         raise ValueError('the operands have {0} and {1} columns'.format(a.cols, b.cols))
@@ -195,7 +203,9 @@ def product(a: Fp8Rows, b: Fp8Rows, bias: Optional[torch.Tensor] = None, relu: b
 def dense(x: torch.Tensor, w: Fp8Rows, bias: Optional[torch.Tensor] = None, relu: bool = False,
           out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """relu(x @ w.T + bias) for x [..., w.cols] in float32 or bfloat16, quantised on the way; out_dtype: x's by default.
-    No gradient (`linear` has one)."""
+    No gradient (`linear` has one): an x or a bias that requires one is refused while gradients are enabled."""
+    if x.requires_grad or (bias is not None and bias.requires_grad):
+        _no_gradient('dense')
     shape = x.shape
     if len(shape) != 2:
         x = x.reshape(-1, shape[-1])

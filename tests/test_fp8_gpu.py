@@ -444,3 +444,14 @@ def test_operands_at_any_strides(fp8):
         assert torch.equal(fp8.dense(x, v), want) and torch.equal(fp8.dense(x[:3], v), fp8.dense(x[:3], w))
         assert torch.equal(fp8.product(fp8.quantize_rows(x), v), fp8.product(fp8.quantize_rows(x), w))
         assert torch.equal(v.dequantize(), w.dequantize())
+
+
+def test_products_without_a_gradient_are_refused_where_one_is_asked_for(fp8):
+    x, w, b = torch.randn(5, 130, device='cuda'), fp8.quantize_rows(torch.randn(8, 130, device='cuda')), torch.zeros(8, device='cuda')
+    xg, bg = x.clone().requires_grad_(True), b.clone().requires_grad_(True)
+    for bad in (lambda: fp8.dense(xg, w), lambda: fp8.dense(x, w, bg), lambda: fp8.product(fp8.quantize_rows(x), w, bg)):
+        with pytest.raises(ValueError, match='gradient'):
+            bad()
+    with torch.no_grad():
+        assert torch.equal(fp8.dense(xg, w, bg), fp8.dense(x, w, b))
+    assert torch.equal(fp8.dense(xg.detach(), w, bg.detach()), fp8.dense(x, w, b))

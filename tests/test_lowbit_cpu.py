@@ -161,6 +161,19 @@ def test_generator_defaults_are_the_reference_ones():
     assert (Conv1dTextVAE.vae_optimizer, Conv1dTextVAE.generator_optimizer, Conv1dTextVAE.generator_products) == ('nadam', 'rmsprop', 'f32')
 
 
+def test_products_without_a_gradient_are_refused_where_one_is_asked_for():
+    from conv1d_text_vae_amd import fp8
+    x, b = torch.zeros(4, 130), torch.zeros(8)
+    w = fp8.Fp8Rows(torch.zeros(8, 256).to(torch.float8_e4m3fn), torch.full((2, 16), 127, dtype=torch.uint8), 130)
+    xg, bg = x.clone().requires_grad_(True), b.clone().requires_grad_(True)
+    calls = (lambda: fp8.dense(xg, w), lambda: fp8.dense(x, w, bg), lambda: fp8.product(w, w, bg))
+    for f in calls:
+        with pytest.raises(ValueError, match='gradient'):
+            f()
+        with torch.no_grad(), pytest.raises(L.C1VError):                  # (and then for want of a GPU)
+            f()
+
+
 def test_estimator_keeps_its_choices_when_pickled():
     """Unfitted and fitted; a fitted one serves as it was fitted, whatever was chosen since; states of before load as they did."""
     import copy
