@@ -841,8 +841,11 @@ struct Fp8Plan { int tile; int splits; };
 //   2048 x 1300 x 640    64: 10.3  128: 10.1  256: 20      2048 x 4096 x 16384   128: 234   256: 306 (half the chip)
 //   2048 x 2048 x 2048   64: 29    128: 21    256: 44      8192 x 8192 x 8192    128: 890   256: 808
 // The 128 / 256 choice compares rounds of workgroups times steps (1.7 us a step with 512 slots, 3.0 us with 256) plus 6 / 8 us
-// a round.  A long K of few tiles is cut into up to four runs whose fp32 sums a second launch adds in order (512 x 512 x 8192:
-// 32 us whole, 14.5 us in four; 512 x 1024 x 8192: 32 us whole, 21.5 in two).
+// a round.  A long K of few tiles is cut into runs whose fp32 sums a second launch adds in order (us, whole / two / four):
+//   256 x 512, 12 blocks 8.2 / 7.6 / 7.2    512 x 512, 12 blocks 8.3 / 8.2 / 8.3     512 x 1024, 16 blocks 10.3 / 10.6 / 12.1
+//              16 blocks 10.0 / 8.5 / 7.8              16 blocks 10.1 / 9.2 / 8.7                 20 blocks 12.0 / 11.5 / 12.6
+//              64 blocks 32 / 19.5 / 13.3              64 blocks 32 / 20.5 / 14.5                 64 blocks 32 / 21.5 / 19.4
+//   768 x 1024, 32 blocks 17.6 / 18.8 / 18.8 (192 tiles; 48 blocks 25 / 22.5 / 22.3)
 static Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t kp) {
     const int64_t nk = kp / FB;
     const int64_t t64 = c1v_cdiv(m, 64) * c1v_cdiv(n, 64), t128 = c1v_cdiv(m, 128) * c1v_cdiv(n, 128), t256 = c1v_cdiv(m, 256) * c1v_cdiv(n, 256);
@@ -852,7 +855,7 @@ static Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t kp) {
         p.tile = c256 < c128 ? 2 : 1;
         return p;
     }
-    if (nk >= 32 && t64 <= 128) p.splits = t64 <= 64 ? 4 : 2;
+    if (t64 <= 64 ? nk >= 16 : t64 <= 128 && nk >= 20) p.splits = t64 <= 64 ? 4 : 2;
     return p;
 }
 
@@ -981,10 +984,13 @@ __global__ __launch_bounds__(64 * NW) void fp8_rows_kernel(Fp8RowsDev d) {
 }
 // Whether x is quantised inside the product's launch.  Up to 16 rows always.  Beyond, a workgroup's K is walked eight blocks at
 // a time and x is quantised again for every 16 to 64 columns, against two launches and 64 x 64 tiles that walk K one block at
-// a time.  Measured (us, f32 / bf16 x, back to back):
-//   256 x 512 x 1920   7.9 / 6.4 here, 12.0 / 12.0 in two launches    512 x 512 x 512    4.7 / 4.1,  6.7 / 6.8
-//   256 x 1024 x 1024  6.4 / 5.4,      8.5 / 8.5                      4096 x 64 x 302    4.8 / 4.7,  6.8 / 7.0
-//   1024 x 1024 x 302  15.6 / 14.7,    6.9 / 7.0 (1024 workgroups)    256 x 512 x 4096   13.9 / 10.0, 12.6 / 12.4 (32 blocks of K)
+// a time.  Measured (us, f32 / bf16 x, back to back), here, and in two launches:
+//   256 x 512 x 1920   8.1 / 6.6,    11.9 / 12.0      512 x 512 x 512    4.7 / 4.1,    6.7 / 6.8
+//   256 x 1024 x 1024  6.4 / 5.4,    8.5 / 8.5        4096 x 64 x 302    4.8 / 4.7,    6.8 / 7.0
+//   1024 x 1024 x 302  15.6 / 14.7,  6.9 / 7.0        512 x 1024 x 302   8.3 / 8.3,    6.6 / 6.7   (1024 and 512 workgroups)
+// With longer K the two launches, which cut it into runs, come nearer: 512 x 512 at 16 blocks 10.9 / 8.7, 11.9 / 11.8; 17 blocks
+// 11.4 / 9.7, 12.6 / 12.5; 20 blocks 12.8 / 10.7, 13.2 / 13.0; 27 blocks 16.4 / 13.1, 14.5 / 14.3.  At two
+// turns of eight blocks no shape loses by the one launch (beyond it few rows would still gain, 64 x 512 at 17 blocks 4 us).
 static bool fp8_dense_direct(int64_t m, int64_t n, int64_t kp) {
     return m <= C1V_FP8_ROWS || (c1v_cdiv(m, 16) * c1v_cdiv(n, 64) <= 256 && kp <= 16 * FB);
 }
@@ -995,18 +1001,20 @@ static void launch_rows1(const Fp8RowsDev& d, hipStream_t st) {
     const dim3 grid((unsigned)c1v_cdiv(d.p.n, 16 * F), (unsigned)c1v_cdiv(d.rows, 16));
     hipLaunchKernelGGL((fp8_rows_kernel<T, F, 8>), grid, dim3(512), 0, st, d);
 }
-// One fragment column per workgroup gives the most workgroups, two or four share the work of quantising x and its reads.
-// Measured for up to 16 rows (us, bf16 x, weights from memory):
-//   13 x 8192 x 4096   1: 15.0   2: 11.1   4: 15.0      4 x 8192 x 8192   1: 21.5   2: 18.6   4: 25.0
-//   16 x 4096 x 4096   1: 9.0    2: 10.4   4: 14.7      1 x 1024 x 1024   1: 3.2    2: 3.6    4: 4.8
-// (sixteen waves instead of eight: no faster anywhere).  Beyond 16 rows the fewest that keep to one workgroup per CU (f32 x):
-//   64 x 512 x 1920    1: 6.6    2: 7.7    4: 9.5       256 x 512 x 1920  1: 11.2   2: 8.1    4: 9.8
-//   17 x 4096 x 1024   1: 5.6    2: 5.1    4: 6.1       512 x 512 x 512   1: 7.3    2: 6.2    4: 4.5
+// One fragment column per workgroup gives the most workgroups, two or four share the work of quantising x and its reads: the fewest
+// that keep to one workgroup per CU.  Measured (us, bf16 / f32 x, weights from memory for up to 16 rows), 1 / 2 / 4:
+//   13 x 4096 x 1024   4.3 4.6 5.6 / 4.8 5.3 6.3       8 x 4112 x 1024    4.5 4.4 5.3 / 5.6 4.9 5.9
+//   1 x 4096 x 4096    8.3 8.8 12.6 / 9.1 10.3 14.3    1 x 4112 x 4096    10.0 8.9 12.6 / 11.9 10.4 14.3
+//   1 x 8192 x 4096    12.6 10.7 13.1 / 13.8 12.2 15.0 1 x 8208 x 4096    14.7 14.4 13.2 / 17.7 18.2 15.0
+//   13 x 8192 x 4096   15.2 11.5 15.0 / 19.9 14.6 17.3 13 x 12288 x 4096  21.2 18.6 15.5 / 27.1 25.2 18.4
+//   64 x 512 x 1920    5.2 6.2 8.0 / 6.6 7.8 9.7       256 x 512 x 1920   8.0 6.4 8.1 / 11.2 7.9 9.7
+//   17 x 4096 x 1024   4.7 4.3 5.3 / 5.7 5.2 6.2       512 x 512 x 512    5.9 4.4 4.1 / 7.6 6.3 4.7
+// (sixteen waves instead of eight: no faster anywhere).
 template <typename T>
 static void launch_rows(const Fp8RowsDev& d, hipStream_t st) {
     const int64_t rt = c1v_cdiv(d.rows, 16);
-    if (d.rows <= C1V_FP8_ROWS ? d.p.n < 6144 : rt * c1v_cdiv(d.p.n, 16) <= 256) launch_rows1<T, 1>(d, st);
-    else if (d.rows <= C1V_FP8_ROWS || rt * c1v_cdiv(d.p.n, 32) <= 256) launch_rows1<T, 2>(d, st);
+    if (rt * c1v_cdiv(d.p.n, 16) <= 256) launch_rows1<T, 1>(d, st);
+    else if (rt * c1v_cdiv(d.p.n, 32) <= 256) launch_rows1<T, 2>(d, st);
     else launch_rows1<T, 4>(d, st);
 }
 

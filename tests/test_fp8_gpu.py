@@ -455,3 +455,21 @@ def test_products_without_a_gradient_are_refused_where_one_is_asked_for(fp8):
     with torch.no_grad():
         assert torch.equal(fp8.dense(xg, w, bg), fp8.dense(x, w, b))
     assert torch.equal(fp8.dense(xg.detach(), w, bg.detach()), fp8.dense(x, w, b))
+
+
+@pytest.mark.parametrize('m', [1, 16, 33])
+@pytest.mark.parametrize('n', [1360, 1376, 2736, 4096, 4097, 8192, 8200])
+def test_column_fragments_of_a_served_product(fp8, m, n):
+    """One, two and four fragments a workgroup on both sides of their borders, with bias, at a K whose last block is not whole."""
+    a, b, want = cancelling(m, n, 300, m + n)
+    bias = torch.from_numpy(np.random.RandomState(n).randint(-9, 10, n).astype(np.float32)).cuda()
+    for x in (a, a.bfloat16()):
+        assert torch.equal(fp8.dense(x, fp8.quantize_rows(b), bias, out_dtype=torch.float32), (want + bias).float())
+
+
+@pytest.mark.parametrize('m,n,k', [(512, 512, 1920), (512, 512, 2048), (66, 130, 2100), (640, 770, 2560), (640, 770, 2432)])
+def test_a_k_in_runs_on_both_sides_of_its_borders(fp8, m, n, k):
+    a, b, want = cancelling(m, n, k, m + k)
+    qa, qb = fp8.quantize_rows(a), fp8.quantize_rows(b)
+    for t in KIND.values():
+        assert torch.equal(fp8.product(qa, qb, out_dtype=t), want.float().to(t))

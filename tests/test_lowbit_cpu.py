@@ -161,6 +161,15 @@ def test_generator_defaults_are_the_reference_ones():
     assert (Conv1dTextVAE.vae_optimizer, Conv1dTextVAE.generator_optimizer, Conv1dTextVAE.generator_products) == ('nadam', 'rmsprop', 'f32')
 
 
+def test_workspace_of_a_k_in_runs():
+    """Partial sums [runs][m][n rounded up to 4] in fp32, exactly: four runs up to 64 tiles of 64 x 64 and from 16 blocks of K,
+    two up to 128 tiles and from 20 blocks, none for more tiles, a shorter K or the larger tiles."""
+    work = L.load().c1v_fp8_gemm_work
+    for m, n, blocks, runs in ((512, 512, 64, 4), (512, 512, 16, 4), (512, 512, 15, 1), (66, 130, 34, 4), (1, 1, 16, 4), (64 * 64, 64, 16, 4), (64 * 64 + 1, 64, 19, 1),
+                               (64 * 64 + 1, 64, 20, 2), (512, 1024, 20, 2), (512, 1021, 33, 2), (512, 1025, 64, 1), (768, 1024, 64, 1), (8192, 8192, 64, 1)):
+        assert work(m, n, 128 * blocks) == (runs * m * (-(-n // 4) * 4) * 4 if runs > 1 else 0), (m, n, blocks)
+
+
 def test_products_without_a_gradient_are_refused_where_one_is_asked_for():
     from conv1d_text_vae_amd import fp8
     x, b = torch.zeros(4, 130), torch.zeros(8)
