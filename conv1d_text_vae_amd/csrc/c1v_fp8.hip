@@ -366,7 +366,7 @@ static int quant_check(const c1v_fp8_quant_args* a, QuantDev& d) {
     C1V_REQUIRE((a->q != nullptr) == (a->s != nullptr) && (a->qt != nullptr) == (a->st != nullptr) && (a->q || a->qt), "fp8_quantize: values and scales go together, one pair at least");
     C1V_REQUIRE(((uintptr_t)a->q | (uintptr_t)a->s | (uintptr_t)a->qt | (uintptr_t)a->st) % 16 == 0, "fp8_quantize: outputs must be 16-byte aligned");
     C1V_REQUIRE(!a->colsum || (a->qt && a->colsum_part), "fp8_quantize: colsum needs qt and colsum_part");
-    C1V_REQUIRE(a->rows < (1ll << 28) && a->cols <= (1ll << 22), "fp8_quantize: too large");
+    C1V_REQUIRE(a->rows <= (1ll << 28) - 16 && a->cols <= (1ll << 22), "fp8_quantize: too large");       // 16 rows, 256 threads: below 2^32 of them
     d = QuantDev{};
     d.x = a->x; d.rows = a->rows; d.cols = a->cols; d.ld = a->ld;
     d.q = (uint8_t*)a->q; d.s = (uint8_t*)a->s; d.kp = c1v_cdiv(a->cols, FB) * FB; d.sp = up16(a->rows);
@@ -1095,7 +1095,7 @@ LinearBufs linear_bwd_bufs(const c1v_fp8_linear_args* a, void* keep, void* temp)
 int linear_check(const c1v_fp8_linear_args* a, const char* what) {
     C1V_REQUIRE(a, "%s: null argument", what);
     C1V_REQUIRE(a->rows > 0 && a->k > 0 && a->n > 0, "%s: bad shape rows=%lld k=%lld n=%lld", what, (long long)a->rows, (long long)a->k, (long long)a->n);
-    C1V_REQUIRE(a->rows <= (1ll << 24) - FB || (!a->need_dk && a->rows < (1ll << 28)), "%s: too many rows (%lld; the kernel's gradient takes up to 2^24 - 128)", what, (long long)a->rows);
+    C1V_REQUIRE(a->rows <= (1ll << 24) - FB || (!a->need_dk && a->rows <= (1ll << 28) - 16), "%s: too many rows (%lld; the kernel's gradient takes up to 2^24 - 128)", what, (long long)a->rows);
     C1V_REQUIRE(a->k <= (1ll << 22) && a->n <= (1ll << 22), "%s: too large", what);
     C1V_REQUIRE((a->x_dtype == C1V_F32 || a->x_dtype == C1V_BF16) && (a->k_dtype == C1V_F32 || a->k_dtype == C1V_BF16), "%s: bad dtype", what);
     C1V_REQUIRE(((uintptr_t)a->keep | (uintptr_t)a->temp) % 16 == 0, "%s: keep and temp must be 16-byte aligned", what);

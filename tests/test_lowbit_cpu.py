@@ -161,6 +161,20 @@ def test_generator_defaults_are_the_reference_ones():
     assert (Conv1dTextVAE.vae_optimizer, Conv1dTextVAE.generator_optimizer, Conv1dTextVAE.generator_products) == ('nadam', 'rmsprop', 'f32')
 
 
+def test_the_largest_number_of_rows_fits_a_launch():
+    """2^28 - 16 rows are 2^24 - 1 workgroups of 256 threads; one more row would be 2^32 threads, which no launch takes."""
+    lib = L.load()
+    mem = (C.c_char * 4096)()
+    p = (C.addressof(mem) + 255) & ~255
+    for rows in ((1 << 28) - 15, (1 << 28) - 1):
+        assert lib.c1v_fp8_quantize(C.byref(L.Fp8QuantArgs(x=p, dtype=0, rows=rows, cols=8, ld=8, q=p, s=p)), None) != 0
+        assert b'large' in lib.c1v_last_error()
+        a = L.Fp8LinearArgs(rows=rows, k=8, n=8, need_dx=1)
+        assert lib.c1v_fp8_linear_sizes(C.byref(a), *(C.byref(C.c_int64()) for _ in range(3))) != 0 and b'rows' in lib.c1v_last_error()
+    a = L.Fp8LinearArgs(rows=(1 << 28) - 16, k=8, n=8, need_dx=1)
+    assert lib.c1v_fp8_linear_sizes(C.byref(a), *(C.byref(C.c_int64()) for _ in range(3))) == 0
+
+
 def test_workspace_of_a_k_in_runs():
     """Partial sums [runs][m][n rounded up to 4] in fp32, exactly: four runs up to 64 tiles of 64 x 64 and from 16 blocks of K,
     two up to 128 tiles and from 20 blocks, none for more tiles, a shorter K or the larger tiles."""
