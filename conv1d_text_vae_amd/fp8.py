@@ -85,7 +85,8 @@ class Fp8Rows:
     def dequantize(self) -> torch.Tensor:
         """float32 [rows, cols]"""
         s = (self.scale[:, :self.rows].to(torch.int32) << 23).view(torch.float32).t()
-        return (self.data.float().view(self.rows, -1, BLOCK) * s.unsqueeze(-1)).view(self.rows, -1)[:, :self.cols]
+        kp = self.data.shape[1]
+        return (self.data.float().view(self.rows, kp // BLOCK, BLOCK) * s.unsqueeze(-1)).view(self.rows, kp)[:, :self.cols]
 
 
 def _empty(rows: int, cols: int, device) -> Tuple[torch.Tensor, torch.Tensor]:

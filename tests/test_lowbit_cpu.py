@@ -184,6 +184,13 @@ def test_workspace_of_a_k_in_runs():
         assert work(m, n, 128 * blocks) == (runs * m * (-(-n // 4) * 4) * 4 if runs > 1 else 0), (m, n, blocks)
 
 
+def test_an_operand_without_rows_or_columns():
+    from conv1d_text_vae_amd import fp8
+    e4 = lambda *s: torch.zeros(s, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    assert fp8.Fp8Rows(e4(0, 256), torch.zeros(2, 0, dtype=torch.uint8), 130).dequantize().shape == (0, 130)
+    assert fp8.Fp8Rows(e4(5, 0), torch.zeros(0, 16, dtype=torch.uint8), 0).dequantize().shape == (5, 0)
+
+
 def test_products_without_a_gradient_are_refused_where_one_is_asked_for():
     from conv1d_text_vae_amd import fp8
     x, b = torch.zeros(4, 130), torch.zeros(8)
