@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import numbers
 from array import array
 from operator import attrgetter
 from typing import Dict, List, Optional, Sequence, Union
@@ -46,7 +47,7 @@ class AdamW:
         self.params: List[torch.Tensor] = list(params)
         if not self.params:
             raise ValueError('there are no parameters')
-        decay = [float(weight_decay)] * len(self.params) if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
+        decay = [float(weight_decay)] * len(self.params) if isinstance(weight_decay, numbers.Real) else [float(w) for w in weight_decay]
         if len(decay) != len(self.params):
             raise ValueError('weight_decay has {0} values for {1} parameters'.format(len(decay), len(self.params)))
         if states not in ('f32', '8bit'):

@@ -191,6 +191,16 @@ def test_an_operand_without_rows_or_columns():
     assert fp8.Fp8Rows(e4(5, 0), torch.zeros(0, 16, dtype=torch.uint8), 0).dequantize().shape == (5, 0)
 
 
+def test_one_weight_decay_of_any_number_type():
+    from conv1d_text_vae_amd import optim
+    for wd in (0.1, 1, np.float32(0.1), np.float64(0.1), np.int64(1)):
+        with pytest.raises(L.C1VError):                                   # (taken, and then no GPU)
+            optim.AdamW([torch.zeros(3), torch.zeros(2)], weight_decay=wd)
+    for wd in (np.float32('nan'), np.float32(-1), [np.float32(0.1)]):
+        with pytest.raises(ValueError):
+            optim.AdamW([torch.zeros(3), torch.zeros(2)], weight_decay=wd)
+
+
 def test_products_without_a_gradient_are_refused_where_one_is_asked_for():
     from conv1d_text_vae_amd import fp8
     x, b = torch.zeros(4, 130), torch.zeros(8)
