@@ -120,10 +120,9 @@ class Seq2SeqGenerator:
         b = None if bias is None else bias[lo:hi]
         if self.products == 'fp8':
             from . import fp8
-            if torch.is_grad_enabled():
+            if train or torch.is_grad_enabled():
                 return fp8.linear(x, W[:, lo:hi], b)
-            if not train:
-                return fp8.dense(x, self._weights8(name, lo, hi, held), None if b is None else b.detach())
+            return fp8.dense(x, self._weights8(name, lo, hi, held), None if b is None else b.detach())
         y = torch.matmul(x, W[:, lo:hi])
         return y if b is None else y + b
 

@@ -240,6 +240,14 @@ def test_generator_8bit_weights_per_stream_update_and_graph():
         assert all(torch.equal(a, b) for a, b in zip(out, again))
 
 
+def test_generator_training_loss_without_gradients_is_the_same():
+    """The training form (dropout, whole-sequence products in 8 bits) under no_grad: the loss of the same seed, to the bit."""
+    words, cin, cout = sentences(seed=4)
+    with_graph = generator().loss(words, cin, cout, train=True)
+    with torch.no_grad():
+        assert torch.equal(generator().loss(words, cin, cout, train=True), with_graph.detach())
+
+
 def test_generator_8bit_inference_sees_every_change_of_its_weights():
     """Updates that the tensors' version counters do not tell -- a replayed optimizer step, a write through `.data`, a replaced
     `.data` -- between decoded characters: each time the answers of a fresh generator with the same weights."""
