@@ -6,8 +6,9 @@
 //
 // Bound by memory: 28 bytes a weight with fp32 states and gradients, 16 with 8-bit states (4 of p read and 4 written, 4 of g,
 // 1 + 1 of each state and 4 bytes of scales per 128).  The clip reads g a second time, before (its norm is not known earlier).
-// Measured, 160 M weights (a copy of 1 GiB reaches 5.1 TB/s): fp32 states 840 us = 5.3 TB/s; 8-bit states with bf16 gradients
-// 422 us = 5.3 TB/s, and 68 us for the clip's norm (4.7 TB/s).  0.2 M weights in 12 tensors: 5.2 and 4 us.
+// Measured, 160 M weights (a copy of 1 GiB reaches 5.1 TB/s): fp32 states 837 us = 5.3 TB/s; 8-bit states with bf16 gradients
+// 422 us = 5.3 TB/s, with the clip 490 us: 92 for the norm (3.5 TB/s) and 395 for the update, which then finds some of g in the
+// last-level cache.  8-bit states with parameters and gradients in bf16 355 us.  0.2 M weights in 12 tensors: 5.2 and 4 us.
 //
 // States in 8 bits.  A block of 128 elements shares a power-of-two scale for m and one for v; m is e4m3, v (never negative) a
 // byte of five exponent and three mantissa bits.  Both are rounded STOCHASTICALLY from m' and v' in fp32 (the update uses the
@@ -284,7 +285,7 @@ __global__ __launch_bounds__(256) void adamw_update_kernel(AdamwDev d) {
             m[0] = a.x; m[1] = a.y; m[2] = a.z; m[3] = a.w; m[4] = b.x; m[5] = b.y; m[6] = b.z; m[7] = b.w;
             v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
         }
-        const float keep = 1.0f - lr * T.weight_decay;
+        const float keep = 1.0f - lr * T.weight_decay, ibc2_up = ibc2 * 0x1p64f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
 #pragma clang fp contract(off)
@@ -293,8 +294,10 @@ __global__ __launch_bounds__(256) void adamw_update_kernel(AdamwDev d) {
             m[k] = a + b;
             const float q = gk * gk, x = v[k] * d.b2, y = q * d.omb2;
             v[k] = x + y;
-            // square root and reciprocal to 1 ulp (v_sqrt_f32, v_rcp_f32): the update term is off by less than 2^-20 of itself
-            const float den = __builtin_amdgcn_sqrtf(v[k] * ibc2) + d.eps;
+            // square root and reciprocal to 1 ulp (v_sqrt_f32, v_rcp_f32): the update term is off by less than 2^-20 of itself.
+            // v_sqrt_f32 takes denormal numbers for zero (an update of m / eps): small v are moved up by 2^64 before
+            const bool low = v[k] < 0x1p-96f;
+            const float den = __builtin_amdgcn_sqrtf(v[k] * (low ? ibc2_up : ibc2)) * (low ? 0x1p-32f : 1.f) + d.eps;
             p[k] = p[k] * keep - (m[k] * step) * __builtin_amdgcn_rcpf(den);
         }
         store8(d.p[ti], i, left, pb, p);
@@ -400,7 +403,8 @@ extern "C" int c1v_adamw_step(const c1v_adamw_args* a, void* stream) {
                 const bool clip = a->clipnorm > 0.f;
                 if (!clip && k > 0) break;
                 // few chunks: up to AW_FEW workgroups, whose sums the update adds up itself; many: up to AW_PART, eight chunks at a time
-                // (bf16 gradients of 160 M weights: 71 us; 2048 workgroups with a share each 86, four chunks at a time 88)
+                // (160 M weights, bf16 gradients, what the clip adds to a step: 71 us; 2048 workgroups with a share each 86, four
+                // chunks at a time 88)
                 d.run = (int)c1v_cdiv(d.chunks, AW_FEW);
                 d.run = d.run < 1 ? 1 : d.run > 8 ? 8 : d.run;
                 const int runs = (int)c1v_cdiv(d.chunks, d.run);

@@ -402,3 +402,21 @@ def test_states_beside_moments_that_are_no_numbers(optim, states):
         assert np.array_equal(np.isnan(got), np.isnan(want))
         fine = np.isfinite(want)
         assert fine.sum() >= n - len(bad) and (np.abs(got - want)[fine] <= tol[fine]).all()
+
+
+@pytest.mark.parametrize('states', ['f32', '8bit'])
+def test_second_moments_among_the_denormal_numbers_and_a_tiny_eps(optim, states):
+    """eps at its lower limit, gradients whose squares are denormal or vanish: the update divides by the root of the held v, not by
+    eps alone.  v / (1 - b2^t) is rounded to a multiple of 2^-149 there, off by 2^-150, which the root passes on by half."""
+    g = torch.from_numpy((10.0 ** np.linspace(-24, -16, 256)).astype(np.float32)).cuda()
+    opt = optim.AdamW([torch.zeros(256, device='cuda')], lr=1.0, weight_decay=0.0, states=states, eps=1e-30)
+    for t in range(1, 4):
+        before, p0 = held(opt)[0], f64(opt.params[0])
+        opt.step([g])
+        m, v = O.moments(before[0], before[1], f32(g), np.float32(1.0), *opt.betas)
+        m, v = m.astype(np.float64), v.astype(np.float64)
+        x = v / (1 - 0.999 ** t)
+        u = (m / (1 - 0.9 ** t)) / (np.sqrt(x) + opt.eps)
+        want = p0 - u
+        tol = 4 * 2.0 ** -24 * np.abs(p0) + (10 * 2.0 ** -23 + 2.0 ** -150 / np.maximum(x, 2.0 ** -149)) * np.abs(u) + 2.0 ** -150 / opt.eps
+        assert (np.abs(f64(opt.params[0]) - want) <= tol).all(), np.abs(f64(opt.params[0]) - want).max()
