@@ -842,10 +842,13 @@ struct Fp8Plan { int tile; int splits; };
 //   2048 x 2048 x 2048   64: 29    128: 21    256: 44      8192 x 8192 x 8192    128: 890   256: 808
 // The 128 / 256 choice compares rounds of workgroups times steps (1.7 us a step with 512 slots, 3.0 us with 256) plus 6 / 8 us
 // a round.  A long K of few tiles is cut into runs whose fp32 sums a second launch adds in order (us, whole / two / four):
-//   256 x 512, 12 blocks 8.2 / 7.6 / 7.2    512 x 512, 12 blocks 8.3 / 8.2 / 8.3     512 x 1024, 16 blocks 10.3 / 10.6 / 12.1
-//              16 blocks 10.0 / 8.5 / 7.8              16 blocks 10.1 / 9.2 / 8.7                 20 blocks 12.0 / 11.5 / 12.6
-//              64 blocks 32 / 19.5 / 13.3              64 blocks 32 / 20.5 / 14.5                 64 blocks 32 / 21.5 / 19.4
+//   256 x 512, 16 blocks 10.0 / 8.5 / 7.8    512 x 512, 16 blocks 10.1 / 9.2 / 8.7     512 x 1024, 16 blocks 10.3 / 10.6 / 12.1
+//              32 blocks 17.3 / 12.1 / 9.6              32 blocks 17.5 / 12.7 / 10.6               32 blocks 17.4 / 14.3 / 15.3
+//              64 blocks 32 / 19.5 / 13.3               64 blocks 32 / 20.5 / 14.5                 64 blocks 32 / 21.5 / 19.4
 //   768 x 1024, 32 blocks 17.6 / 18.8 / 18.8 (192 tiles; 48 blocks 25 / 22.5 / 22.3)
+// A product by itself would be ahead in runs from 16 blocks; they start at 32 because a training layer's two products share a launch
+// only whole (backward of 2048 x 302 -> 128: 15.3 us together, 17.5 apart with runs; 3000 rows 19.9 / 19.2, 4096 rows 23.6 / 20.1)
+// and a gradient has to have the same bits whichever others are asked for.
 static Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t kp) {
     const int64_t nk = kp / FB;
     const int64_t t64 = c1v_cdiv(m, 64) * c1v_cdiv(n, 64), t128 = c1v_cdiv(m, 128) * c1v_cdiv(n, 128), t256 = c1v_cdiv(m, 256) * c1v_cdiv(n, 256);
@@ -855,7 +858,7 @@ static Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t kp) {
         p.tile = c256 < c128 ? 2 : 1;
         return p;
     }
-    if (t64 <= 64 ? nk >= 16 : t64 <= 128 && nk >= 20) p.splits = t64 <= 64 ? 4 : 2;
+    if (nk >= 32 && t64 <= 128) p.splits = t64 <= 64 ? 4 : 2;
     return p;
 }
 
@@ -988,9 +991,9 @@ __global__ __launch_bounds__(64 * NW) void fp8_rows_kernel(Fp8RowsDev d) {
 //   256 x 512 x 1920   8.1 / 6.6,    11.9 / 12.0      512 x 512 x 512    4.7 / 4.1,    6.7 / 6.8
 //   256 x 1024 x 1024  6.4 / 5.4,    8.5 / 8.5        4096 x 64 x 302    4.8 / 4.7,    6.8 / 7.0
 //   1024 x 1024 x 302  15.6 / 14.7,  6.9 / 7.0        512 x 1024 x 302   8.3 / 8.3,    6.6 / 6.7   (1024 and 512 workgroups)
-// With longer K the two launches, which cut it into runs, come nearer: 512 x 512 at 16 blocks 10.9 / 8.7, 11.9 / 11.8; 17 blocks
-// 11.4 / 9.7, 12.6 / 12.5; 20 blocks 12.8 / 10.7, 13.2 / 13.0; 27 blocks 16.4 / 13.1, 14.5 / 14.3.  At two
-// turns of eight blocks no shape loses by the one launch (beyond it few rows would still gain, 64 x 512 at 17 blocks 4 us).
+//   256 x 512 x 2048   8.2 / 6.6,    12.3 / 12.5      256 x 512 x 2560   9.3 / 7.6,    14.4 / 14.5
+//   256 x 512 x 4096   13.9 / 10.0,  12.6 / 12.4      128 x 512 x 4096   11.7 / 8.1,   11.4 / 11.4    (K in runs in two launches)
+// At two turns of eight blocks no shape loses by the one launch; it would still be ahead up to 31 blocks.
 static bool fp8_dense_direct(int64_t m, int64_t n, int64_t kp) {
     return m <= C1V_FP8_ROWS || (c1v_cdiv(m, 16) * c1v_cdiv(n, 64) <= 256 && kp <= 16 * FB);
 }

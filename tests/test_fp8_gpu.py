@@ -467,9 +467,26 @@ def test_column_fragments_of_a_served_product(fp8, m, n):
         assert torch.equal(fp8.dense(x, fp8.quantize_rows(b), bias, out_dtype=torch.float32), (want + bias).float())
 
 
-@pytest.mark.parametrize('m,n,k', [(512, 512, 1920), (512, 512, 2048), (66, 130, 2100), (640, 770, 2560), (640, 770, 2432)])
+@pytest.mark.parametrize('m,n,k', [(512, 512, 3968), (512, 512, 4096), (66, 130, 3970), (640, 770, 3968), (640, 770, 4096), (640, 900, 4096)])
 def test_a_k_in_runs_on_both_sides_of_its_borders(fp8, m, n, k):
     a, b, want = cancelling(m, n, k, m + k)
     qa, qb = fp8.quantize_rows(a), fp8.quantize_rows(b)
     for t in KIND.values():
         assert torch.equal(fp8.product(qa, qb, out_dtype=t), want.float().to(t))
+
+
+@pytest.mark.parametrize('m,n', [(5, 300), (100, 200), (700, 900), (2050, 1300), (4352, 4096)])
+def test_sums_hold_24_bits(fp8, m, n):
+    """One block of K: 448 * 448 and -448 * 448 beside products that are multiples of 2^-6.  Every partial sum, in any order, is a
+    multiple of 2^-6 below 2^18, 24 bits, so fp32 sums are exact and anything shorter is not."""
+    rng = np.random.RandomState(m)
+    a, b = rng.randint(-3, 4, (m, 128)) / 8.0, rng.randint(-3, 4, (n, 128)) / 8.0
+    i, j = rng.choice(128, 2, replace=False)
+    a[:, i] = a[:, j] = b[:, i] = 448.0
+    b[:, j] = -448.0
+    a, b = torch.from_numpy(a.astype(np.float32)).cuda(), torch.from_numpy(b.astype(np.float32)).cuda()
+    want = (a.double() @ b.double().t()).float()
+    qa, qb = fp8.quantize_rows(a), fp8.quantize_rows(b)
+    assert torch.equal(qa.dequantize(), a) and torch.equal(qb.dequantize(), b)
+    assert torch.equal(fp8.product(qa, qb), want) and torch.equal(fp8.dense(a, qb), want)
+    assert torch.equal(fp8.product(qa, qb, out_dtype=torch.bfloat16), want.bfloat16())

@@ -176,11 +176,11 @@ def test_the_largest_number_of_rows_fits_a_launch():
 
 
 def test_workspace_of_a_k_in_runs():
-    """Partial sums [runs][m][n rounded up to 4] in fp32, exactly: four runs up to 64 tiles of 64 x 64 and from 16 blocks of K,
-    two up to 128 tiles and from 20 blocks, none for more tiles, a shorter K or the larger tiles."""
+    """Partial sums [runs][m][n rounded up to 4] in fp32, exactly: from 32 blocks of K four runs up to 64 tiles of 64 x 64 and two
+    up to 128 tiles, none for more tiles, a shorter K or the larger tiles."""
     work = L.load().c1v_fp8_gemm_work
-    for m, n, blocks, runs in ((512, 512, 64, 4), (512, 512, 16, 4), (512, 512, 15, 1), (66, 130, 34, 4), (1, 1, 16, 4), (64 * 64, 64, 16, 4), (64 * 64 + 1, 64, 19, 1),
-                               (64 * 64 + 1, 64, 20, 2), (512, 1024, 20, 2), (512, 1021, 33, 2), (512, 1025, 64, 1), (768, 1024, 64, 1), (8192, 8192, 64, 1)):
+    for m, n, blocks, runs in ((512, 512, 64, 4), (512, 512, 32, 4), (512, 512, 31, 1), (66, 130, 34, 4), (1, 1, 32, 4), (64 * 64, 64, 32, 4), (64 * 64 + 1, 64, 31, 1),
+                               (64 * 64 + 1, 64, 32, 2), (512, 1024, 32, 2), (512, 1021, 33, 2), (512, 1025, 64, 1), (768, 1024, 64, 1), (8192, 8192, 64, 1)):
         assert work(m, n, 128 * blocks) == (runs * m * (-(-n // 4) * 4) * 4 if runs > 1 else 0), (m, n, blocks)
 
 
